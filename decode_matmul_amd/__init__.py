@@ -9,6 +9,9 @@ in the half-precision form of the same code format:
                                                   # grid half [256,8] -> y half [M,N]
     W = decode(codes, grid)                       # dense half [N,K], bit-exact decode
 
+and around the product, for a model's MLP on such weights: `decode_matmul_fused` (bias, activation, gate,
+residual in the epilogue), `decode_matmul_grouped` (the same per expert), `route_experts` and `combine_experts`.
+
 The functions are the compiled PyTorch operator (`_C`, host C++) over the C ABI of
 `libdmm.so` (hand-written HIP).  GPU tensors run the HIP kernels; `decode_matmul` and `decode` also
 take tensors in host memory, which go to the library's own host route (plain C++ loops, the
@@ -16,6 +19,7 @@ counterpart of the reference's CPU path, test_decode_matmul.py:29-71).  Nothing 
 the built extension every operator raises ImportError (the import itself succeeds, so that
 `python -m decode_matmul_amd.build` can run on a fresh tree).
 """
+import collections as _collections
 import os as _os
 
 _PKG_DIR = _os.path.dirname(_os.path.abspath(__file__))
@@ -59,6 +63,11 @@ __all__ = [
     "pack_codes",
     "decode_matmul_packed",
     "decode",
+    "decode_matmul_fused",
+    "decode_matmul_grouped",
+    "route_experts",
+    "combine_experts",
+    "Routing",
     "lib",
     "build_codebook_abs",
     "grid_from_codebook",
@@ -116,3 +125,56 @@ def decode_matmul_packed(x, packed, grid, scale, N):
 def decode(codes, grid):
     """Dense half matrix W[N,K] from codes[N,K/8]; W[n, 8j+d] is dim d of codes[n, j]."""
     return _ext().decode(codes, grid)
+
+
+def decode_matmul_fused(x, codes, grid, scale, *, bias=None, activation="none", gated=False, residual=None, out_dtype=None):
+    """`decode_matmul` with an epilogue, fp32 until one rounding at the store:
+
+        z = scale * x @ decode(codes, grid).T + bias
+        y = act(z) + residual                              gated=False, codes [N, K/8]
+        y = act(z[:, :N]) * z[:, N:] + residual            gated=True, codes [2 N, K/8]: gate rows, then up rows
+
+    x half [M, K]; bias (one value per row of codes) and residual [M, N] half or float32; activation "none",
+    "relu", "silu", "gelu" (erf) or "gelu_tanh"; out_dtype float16 (default) or float32.  scale: a number, or for a gated
+    call a pair (gate, up).  No gradient: an input that requires one is refused."""
+    scale, scale_up = (float(s) for s in scale) if isinstance(scale, (tuple, list)) else (float(scale),) * 2
+    if scale != scale_up and not gated:
+        raise RuntimeError("decode_matmul_fused: a pair of scales is for a gated call")
+    return _ext().decode_matmul_fused(x, codes, grid, scale, scale_up, bias, activation, bool(gated), residual,
+                                      out_dtype or _torch.float16)
+
+
+def decode_matmul_grouped(x, codes, grid, scale, offsets, *, rows=None, bias=None, activation="none", gated=False,
+                          out_dtype=None, out=None):
+    """`decode_matmul_fused` per expert on rows grouped by expert: row p of the result, offsets[e] <= p < offsets[e + 1],
+    is made with codes[e] from x[rows[p]] (rows=None: x[p]).
+
+    codes [E, N, K/8] (gated: [E, 2 N, K/8]), bias [E, ...] one value per row of codes, scale a number, float32 [E], or
+    for a gated call float32 [E, 2]; offsets int32 [E + 1] and rows int32 [R] live on x's device and are not read by the
+    host (`route_experts` makes both).  An entry of rows outside x stands for a row of zeros.  Rows from
+    offsets[E] on are not written: in `out` (optional, [R, N]) they stay as they were, in a result allocated here
+    their content is undefined."""
+    scales = scale if isinstance(scale, _torch.Tensor) else None
+    return _ext().decode_matmul_grouped(x, codes, grid, 1.0 if scales is not None else float(scale), scales, offsets, rows, bias,
+                                        activation, bool(gated), out_dtype or (out.dtype if out is not None else _torch.float16), out)
+
+
+Routing = _collections.namedtuple("Routing", "weights experts offsets rows slots")
+
+
+def route_experts(logits, k, *, scoring="softmax", normalize=True):
+    """The k largest logits of every row of logits [T, E] (half, bfloat16 or float32), equal ones by index, and the lists
+    that `decode_matmul_grouped` and `combine_experts` read.  Returns a `Routing`:
+
+        weights  float32 [T, k]   softmax over the row, or sigmoid, of the chosen; divided by their sum if normalize
+        experts  int32 [T, k]     -1: no choice (a logit of -inf or NaN is never chosen; such a weight is 0)
+        offsets  int32 [E + 1]    first row of every expert, rows sorted by expert, then by token
+        rows     int32 [T * k]    the token of every sorted row; -1 from offsets[E] on
+        slots    int32 [T, k]     the sorted row of every choice; -1: no choice"""
+    return Routing(*_ext().route_experts(logits, int(k), scoring, bool(normalize)))
+
+
+def combine_experts(y, slots, weights, *, residual=None, out_dtype=None):
+    """out[t] = residual[t] + sum over j of weights[t, j] * y[slots[t, j]], in fp32 with one rounding; a slot outside y adds
+    nothing.  y [R, N] half or float32, slots int32 [T, k], weights float32 [T, k], residual [T, N]."""
+    return _ext().combine_experts(y, slots, weights, residual, out_dtype or _torch.float16)

@@ -1,4 +1,4 @@
-"""In-tree build of the native parts: libdmm.so (HIP kernels + C ABI, hipcc, gfx950) and
+"""In-tree build of the native parts: libdmm.so (HIP kernels + C ABI, hipcc, gfx950, two sources) and
 _C.so (the PyTorch operator, host C++ only, g++).  No hipify, no JIT cache: the built files
 sit next to this module so they travel with the tree.
 
@@ -11,6 +11,8 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)
@@ -24,7 +26,6 @@ HIPCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-fPIC",
-    "-shared",
     # scalar fp32 code must not be turned into packed fp32 instructions
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
@@ -48,12 +49,19 @@ def hipcc_path():
     raise RuntimeError("hipcc not found")
 
 
+SOURCES = ("dmm.hip", "dmm_ops.hip")
+
+
 def build_lib(verbose=False):
-    """hipcc: csrc/dmm.hip (which includes the dmm_*.h kernel files beside it) -> libdmm.so
-    (gfx950 code object + the extern "C" entry points)."""
-    cmd = [hipcc_path()] + HIPCC_FLAGS + ["-Rpass-analysis=kernel-resource-usage",
-                                          "-I" + INCLUDE, "-o", LIB_PATH, os.path.join(CSRC, "dmm.hip")]
-    out = _run(cmd)
+    """hipcc: csrc/dmm.hip and csrc/dmm_ops.hip (which include the dmm_*.h kernel files beside them), side by
+    side -> libdmm.so (gfx950 code objects + the extern "C" entry points)."""
+    with tempfile.TemporaryDirectory() as tmp:
+        objs = [os.path.join(tmp, src + ".o") for src in SOURCES]
+        cmds = [[hipcc_path()] + HIPCC_FLAGS + ["-c", "-Rpass-analysis=kernel-resource-usage", "-I" + INCLUDE,
+                                                "-o", obj, os.path.join(CSRC, src)] for src, obj in zip(SOURCES, objs)]
+        with ThreadPoolExecutor(len(cmds)) as pool:
+            out = "\n".join(pool.map(_run, cmds))
+        _run([hipcc_path(), "--offload-arch=gfx950", "-fPIC", "-shared", "-o", LIB_PATH] + objs)
     # No kernel may spill registers to scratch memory: the kernels are sized to their register
     # budget, and a build of the streaming kernel that spilled ran at half speed and returned
     # wrong sums on the GPU.  The compiler's resource remarks name the offender.

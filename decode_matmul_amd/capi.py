@@ -40,6 +40,34 @@ SYMBOLS = {
     "dmm_read_probe": (ctypes.c_int, [_P, _P, _I64, _I64, _P]),
 }
 
+
+
+class Epilogue(ctypes.Structure):
+    """dmm_epilogue of include/dmm.h."""
+    _fields_ = [("bias", _P), ("residual", _P), ("bias_type", ctypes.c_int32), ("residual_type", ctypes.c_int32),
+                ("out_type", ctypes.c_int32), ("activation", ctypes.c_int32), ("gated", ctypes.c_int32),
+                ("scale", _F), ("scale_up", _F)]
+
+
+# the operators around the product
+_INT = ctypes.c_int
+_EP = ctypes.POINTER(Epilogue)
+_GROUPED = [_P, _I64, _P, _P, _P, _P, _INT, _P, _EP, _P, _I64, _I64, _I64, _I64]
+_ROUTE = [_P, _INT, _I64, _I64, _I64, _INT, _INT, _P, _P, _P, _P, _P]
+_COMBINE = [_P, _INT, _P, _P, _P, _INT, _P, _INT, _I64, _I64, _I64, _I64]
+SYMBOLS.update({
+    "dmm_fused_workspace_bytes": (_I64, [_I64, _I64, _I64, _INT]),
+    "dmm_decode_matmul_fused": (_INT, [_P, _P, _P, _EP, _P, _I64, _I64, _I64, _P, _I64, _P]),
+    "dmm_decode_matmul_fused_host": (_INT, [_P, _P, _P, _EP, _P, _I64, _I64, _I64]),
+    "dmm_decode_matmul_grouped": (_INT, _GROUPED + [_P]),
+    "dmm_decode_matmul_grouped_host": (_INT, _GROUPED),
+    "dmm_route_workspace_bytes": (_I64, [_I64, _I64]),
+    "dmm_route_experts": (_INT, _ROUTE + [_P, _I64, _P]),
+    "dmm_route_experts_host": (_INT, _ROUTE),
+    "dmm_combine_experts": (_INT, _COMBINE + [_P]),
+    "dmm_combine_experts_host": (_INT, _COMBINE),
+})
+
 _lib = None
 
 

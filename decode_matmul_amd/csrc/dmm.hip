@@ -12,15 +12,17 @@
 // 16x16x32 / 32x32x16 half MFMA.  Nothing decoded ever goes back through memory on the
 // matrix-vector path.
 //
-// This file is the one translation unit of the library: shared types, then the kernel files
-// beside it (each included once, inside namespace dmm, in dependency order), then the
-// extern "C" entry points.
-//   dmm_tables.h      decode tables, decode of one code, standalone decoder, catch-all operator
+// This file is the library's first translation unit: the kernel files beside it (each included
+// once, inside namespace dmm, in dependency order), then the extern "C" entry points.  The second,
+// dmm_ops.hip, holds the operators around the product.
+//   dmm_types.h, dmm_launch.h, dmm_hostroute.h   shared with dmm_ops.hip: types, launch plumbing, host loops
+//   dmm_tables.h      decode tables, decode of one code
+//   dmm_plain.h       standalone decoder, catch-all operator, split-K reduction
 //   dmm_gemv_f16.h    matrix-vector helpers and the streaming kernel on 16-bit operands
 //   dmm_gemv_q8.h     matrix-vector kernels on 8-bit operands (fp8 weights, bf8 terms of x)
 //   dmm_gemv_q8d.h    batch 1 on 8-bit operands, every tile of a workgroup in registers
 //   dmm_gemv_small.h  small-batch kernel with x in registers
-//   dmm_gemm.h        matrix-matrix kernels and the split-K reduction
+//   dmm_gemm.h        matrix-matrix kernels
 //   dmm_int8.h        the reference's integer operator
 //   dmm_aux.h         offline repack, read probe
 //   dmm_host.h        library scratch memory, launch plumbing, set-up, checks and dispatch
@@ -39,19 +41,11 @@
 
 namespace dmm {
 
-typedef _Float16 half_t;
-typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
-typedef float f16_t __attribute__((ext_vector_type(16)));
-typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
-typedef int i8_t __attribute__((ext_vector_type(8)));
-
-constexpr int kWave = 64;
-
+#include "dmm_types.h"
+#include "dmm_launch.h"
+#include "dmm_hostroute.h"
 #include "dmm_tables.h"
+#include "dmm_plain.h"
 #include "dmm_gemv_f16.h"
 #include "dmm_gemv_q8.h"
 #include "dmm_gemv_q8d.h"

@@ -1,0 +1,205 @@
+// What happens to a finished sum of the operators with an epilogue: scale, bias, activation (plain or
+// gated), residual, one rounding, store.
+// Part of libdmm: included by dmm_ops.hip inside namespace dmm; not a translation unit of its own.
+
+// Everything is in fp32 until the one rounding at the store.  z = scale * sum + bias; a plain call
+// gives act(z), a gated one act(z of row n) * (z of row N + n); then the residual is added.
+struct Epi {
+    const void *bias;       // [E][N], gated [E][2 N]; or null
+    const void *residual;   // [M][N]; or null.  May be y itself: every element is read by the thread that writes it
+    void *y;                // [M][N]
+    const float *scales;    // [E][scale_cols] on the device, on top of scale; or null
+    float scale, scale_up;  // scale_up: rows N .. 2 N - 1 of a gated call
+    int N;
+    int act;
+    int scale_cols;
+    int bias_f32, residual_f32, out_f32;
+    int vec;                // N % 4 == 0 and every pointer aligned for four elements at a time
+};
+
+// 1 / (1 + exp(-z)) to about two units in the last place.  exp(-z) = 2^t (1 + ln 2 * r) with t the rounded product
+// z * -log2(e) and r what that product lost: without r the relative error would grow with |z|.  An exponential that
+// overflows gives 0.
+__device__ __forceinline__ float epi_sigmoid(float z)
+{
+    constexpr float kLog2e = 1.44269502162933349609f, kLog2eLo = 1.92596299112661746887e-8f, kLn2 = 0.693147182464599609375f;
+    const float t = z * -kLog2e;
+    const float r = __builtin_fmaf(z, -kLog2e, -t) - z * kLog2eLo;
+    const float p = __builtin_amdgcn_exp2f(t);
+    const float e = __builtin_fabsf(t) < 127.f ? __builtin_fmaf(p, r * kLn2, p) : p;   // no inf * 0, no inf - inf
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+__device__ __forceinline__ float epi_act(float z, int act)
+{
+    switch (act) {
+        case DMM_ACT_RELU: return z < 0.f ? 0.f : z;   // keeps NaN
+        case DMM_ACT_SILU: return z * epi_sigmoid(z);
+        case DMM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+        // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
+        case DMM_ACT_GELU_TANH: return z * epi_sigmoid(1.59576912160573071176f * __builtin_fmaf(0.044715f * z * z, z, z));
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float epi_load(const void *p, int64_t i, int f32)
+{
+    return f32 ? reinterpret_cast<const float *>(p)[i] : (float)reinterpret_cast<const half_t *>(p)[i];
+}
+
+// four elements from i on, i % 4 == 0 (N % 4 == 0, see Epi::vec)
+__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32)
+{
+    if (f32) return *reinterpret_cast<const f4_t *>(reinterpret_cast<const float *>(p) + i);
+    const h4_t h = *reinterpret_cast<const h4_t *>(reinterpret_cast<const half_t *>(p) + i);
+    return f4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+}
+
+struct EpiScale {
+    float s, up;
+};
+__device__ __forceinline__ EpiScale epi_scale(const Epi &e, int expert)
+{
+    EpiScale r{e.scale, e.scale_up};
+    if (e.scales) {
+        r.s *= e.scales[(int64_t)expert * e.scale_cols];
+        r.up *= e.scales[(int64_t)expert * e.scale_cols + e.scale_cols - 1];
+    }
+    return r;
+}
+
+// one output (row, n): v the sum of row n of W, u that of row N + n (gated)
+template <bool kGated>
+__device__ __forceinline__ void epi_store1(const Epi &e, const EpiScale &sc, float v, float u, int64_t row, int n, int expert)
+{
+    const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
+    float z = v * sc.s;
+    if (e.bias) z += epi_load(e.bias, b, e.bias_f32);
+    z = epi_act(z, e.act);
+    if (kGated) {
+        float w = u * sc.up;
+        if (e.bias) w += epi_load(e.bias, b + e.N, e.bias_f32);
+        z *= w;
+    }
+    const int64_t i = row * e.N + n;
+    if (e.residual) z += epi_load(e.residual, i, e.residual_f32);
+    if (e.out_f32) reinterpret_cast<float *>(e.y)[i] = z;
+    else reinterpret_cast<half_t *>(e.y)[i] = (half_t)z;
+}
+
+// four outputs (row, n .. n + 3), n % 4 == 0; those past N are left out
+template <bool kGated>
+__device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n,
+                                           int expert)
+{
+    if (!e.vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (n + i < e.N) epi_store1<kGated>(e, sc, v[i], u[i], row, n + i, expert);
+        return;
+    }
+    if (n >= e.N) return;
+    const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
+    f4_t z = v * sc.s;
+    if (e.bias) z += epi_load4(e.bias, b, e.bias_f32);
+#pragma unroll
+    for (int i = 0; i < 4; i++) z[i] = epi_act(z[i], e.act);
+    if (kGated) {
+        f4_t w = u * sc.up;
+        if (e.bias) w += epi_load4(e.bias, b + e.N, e.bias_f32);
+        z *= w;
+    }
+    const int64_t i = row * e.N + n;
+    if (e.residual) z += epi_load4(e.residual, i, e.residual_f32);
+    if (e.out_f32) {
+        *reinterpret_cast<f4_t *>(reinterpret_cast<float *>(e.y) + i) = z;
+    } else {
+        h4_t o;
+#pragma unroll
+        for (int k = 0; k < 4; k++) o[k] = (half_t)z[k];
+        *reinterpret_cast<h4_t *>(reinterpret_cast<half_t *>(e.y) + i) = o;
+    }
+}
+
+// ------------------------------------------------------------------ rows by expert
+// offsets[e] .. offsets[e + 1] are expert e's rows of y.  The values come from the device and are not checked
+// on the host: they are cut to 0 <= first <= last <= R, so that no list, however broken, leads a kernel out of
+// its buffers.  No list: one expert with all R rows.
+struct Groups {
+    const int32_t *offsets;   // [E + 1] or null
+    const int32_t *rows;      // [R]: which row of x a row of y is made from; null: the same
+    int E, R, T;              // rows of y, rows of x
+};
+
+struct GroupRange {
+    int lo, hi;
+};
+__device__ __forceinline__ GroupRange group_range(const Groups &g, int e)
+{
+    if (!g.offsets) return GroupRange{0, g.R};
+    const int a = g.offsets[e], b = g.offsets[e + 1];
+    GroupRange r;
+    r.lo = a < 0 ? 0 : a > g.R ? g.R : a;
+    r.hi = b < r.lo ? r.lo : b > g.R ? g.R : b;
+    return r;
+}
+
+// row of x for row p of y, -1 for a row of zeros (an entry of the list that points outside x)
+__device__ __forceinline__ int group_row(const Groups &g, int p)
+{
+    const int t = g.rows ? g.rows[p] : p;
+    return t >= 0 && t < g.T ? t : -1;
+}
+
+// ------------------------------------------------------------------ catch-all
+// One wave per output column (a gated call: per pair of rows of W), lanes stride over the codes, dot products on
+// the vector ALU, as the catch-all of the plain product: any K % 8 == 0, any alignment, sizes past 32-bit offsets.
+// blockIdx.y: the expert.
+template <bool kGated>
+__global__ __launch_bounds__(256) void ops_generic_kernel(const uint16_t *__restrict__ x, const uint16_t *__restrict__ codes,
+                                                          const void *__restrict__ grid, Groups g, Epi epi, int64_t K)
+{
+    constexpr int kMC = 4, kH = kGated ? 2 : 1;
+    __shared__ DecodeTables tab;
+    const int e = blockIdx.y;
+    const GroupRange gr = group_range(g, e);
+    if (gr.lo == gr.hi) return;
+    stage_tables<false>(tab, grid, threadIdx.x, 256);
+    __syncthreads();
+    const int lane = threadIdx.x & 63;
+    const int wave = threadIdx.x >> 6;
+    const int64_t kc = K >> 3, N = epi.N;
+    const uint16_t *ce = codes + (int64_t)e * kH * N * kc;
+    const EpiScale sc = epi_scale(epi, e);
+    for (int64_t n = (int64_t)blockIdx.x * 4 + wave; n < N; n += (int64_t)gridDim.x * 4) {
+        for (int p0 = gr.lo; p0 < gr.hi; p0 += kMC) {
+            const uint16_t *xr[kMC];
+#pragma unroll
+            for (int m = 0; m < kMC; m++) {
+                const int t = p0 + m < gr.hi ? group_row(g, p0 + m) : -1;
+                xr[m] = t >= 0 ? x + (int64_t)t * K : nullptr;
+            }
+            float acc[kH][kMC] = {};
+            for (int64_t j = lane; j < kc; j += kWave) {
+#pragma unroll
+                for (int h = 0; h < kH; h++) {
+                    const u4_t w = decode8(ce[(n + h * N) * kc + j], tab);
+#pragma unroll
+                    for (int m = 0; m < kMC; m++) {
+                        if (!xr[m]) continue;
+#pragma unroll
+                        for (int d = 0; d < 8; d++)
+                            acc[h][m] = __builtin_fmaf((float)__builtin_bit_cast(half_t, xr[m][j * 8 + d]), (float)as_h2(w[d >> 1])[d & 1],
+                                                       acc[h][m]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < kMC; m++) {
+                const float v = wave_sum(acc[0][m]);
+                const float u = kGated ? wave_sum(acc[kH - 1][m]) : 0.f;
+                if (lane == 0 && p0 + m < gr.hi) epi_store1<kGated>(epi, sc, v, u, p0 + m, (int)n, e);
+            }
+        }
+    }
+}

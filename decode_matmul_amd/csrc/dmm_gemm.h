@@ -575,28 +575,3 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
             }
         }
 }
-
-// y = half(scale * sum_z part[z]) over M * N elements; the order of the sum is fixed, so the
-// result does not depend on how the blocks were scheduled.
-__global__ __launch_bounds__(256) void splitk_reduce_kernel(const float *__restrict__ part, uint16_t *__restrict__ y,
-                                                            int64_t mn, int splits, float scale)
-{
-    const int64_t i4 = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i4 >= mn) return;
-    if (i4 + 3 < mn && (mn & 3) == 0) {
-        f4_t sacc = *reinterpret_cast<const f4_t *>(part + i4);
-        for (int z = 1; z < splits; z++) sacc += *reinterpret_cast<const f4_t *>(part + (int64_t)z * mn + i4);
-        u2_t v;
-        v[0] = (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(sacc[0] * scale)) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (half_t)(sacc[1] * scale)) << 16);
-        v[1] = (uint32_t)__builtin_bit_cast(uint16_t, (half_t)(sacc[2] * scale)) |
-               ((uint32_t)__builtin_bit_cast(uint16_t, (half_t)(sacc[3] * scale)) << 16);
-        *reinterpret_cast<u2_t *>(y + i4) = v;
-    } else {
-        for (int64_t i = i4; i < mn && i < i4 + 4; i++) {
-            float sacc = part[i];
-            for (int z = 1; z < splits; z++) sacc += part[(int64_t)z * mn + i];
-            y[i] = __builtin_bit_cast(uint16_t, (half_t)(sacc * scale));
-        }
-    }
-}

@@ -14,29 +14,8 @@ static __device__ __align__(256) unsigned char scratch[kScratchBytes];
 thread_local hipEvent_t tls_start = nullptr;
 thread_local hipEvent_t tls_stop = nullptr;
 
-template <typename T>
-struct same_type { typedef T type; };
-
-// Enqueue one kernel; the status is what the launch call itself returns (no look at the
-// thread's last-error state, which may hold somebody else's stale error).  kFirst / kLast:
-// whether this launch opens / closes the span the timing events bracket (an operator call
-// that takes two kernels records start before the first and stop after the second).
-template <bool kFirst = true, bool kLast = true, typename... KArgs>
-int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t shmem, hipStream_t stream,
-           typename same_type<KArgs>::type... args)
-{
-    void *argv[] = {(void *)&args...};
-    if (tls_start && tls_stop)
-        return (int)hipExtLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, argv, shmem, stream,
-                                       kFirst ? tls_start : nullptr, kLast ? tls_stop : nullptr, 0);
-    return (int)hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, argv, shmem, stream);
-}
-
-inline bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
-
 // ---- per-device state, set up by dmm_init --------------------------------------------------
 constexpr int kMaxDevices = 64;
-constexpr int kLdsMax = 160 * 1024;
 
 struct DeviceState {
     std::atomic<int> ready{0};
@@ -45,18 +24,6 @@ struct DeviceState {
 };
 DeviceState g_dev[kMaxDevices];
 std::mutex g_init_mutex;
-
-// Every kernel that needs more dynamic LDS than the default limit, or whose table addressing
-// assumes that its dynamic LDS starts at LDS address 0 (true exactly when the kernel has no
-// static LDS, which dmm_init verifies from the function's attributes).
-struct KernelInfo {
-    const void *fn;
-    int dynamic_lds;   // bytes to allow; 0 = default limit is enough
-    bool lds_base0;
-};
-
-template <typename... KArgs>
-KernelInfo kinfo(void (*k)(KArgs...), int lds, bool base0) { return KernelInfo{reinterpret_cast<const void *>(k), lds, base0}; }
 
 const std::vector<KernelInfo> &kernel_table()
 {
@@ -145,16 +112,18 @@ int init_current_device(int dev)
     hipError_t e = hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev);
     if (e != hipSuccess) return (int)e;
     ds.cus = v > 0 ? v : 256;
-    for (const KernelInfo &k : kernel_table()) {
-        if (k.lds_base0) {
-            hipFuncAttributes attr;
-            e = hipFuncGetAttributes(&attr, k.fn);
-            if (e != hipSuccess) return (int)e;
-            if (attr.sharedSizeBytes != 0) return DMM_ERR_INTERNAL;
-        }
-        if (k.dynamic_lds > 0) {
-            e = hipFuncSetAttribute(k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, k.dynamic_lds);
-            if (e != hipSuccess) return (int)e;
+    for (const std::vector<KernelInfo> *table : {&kernel_table(), &ops_kernel_table()}) {
+        for (const KernelInfo &k : *table) {
+            if (k.lds_base0) {
+                hipFuncAttributes attr;
+                e = hipFuncGetAttributes(&attr, k.fn);
+                if (e != hipSuccess) return (int)e;
+                if (attr.sharedSizeBytes != 0) return DMM_ERR_INTERNAL;
+            }
+            if (k.dynamic_lds > 0) {
+                e = hipFuncSetAttribute(k.fn, hipFuncAttributeMaxDynamicSharedMemorySize, k.dynamic_lds);
+                if (e != hipSuccess) return (int)e;
+            }
         }
     }
     void *p = nullptr;
@@ -168,7 +137,7 @@ int init_current_device(int dev)
 // Called by every entry point that launches, after its argument checks.  A first call on a
 // device does the set-up unless the stream is being captured into a graph, where host-side
 // set-up has no business: such a caller runs dmm_init beforehand.
-int ensure_ready(hipStream_t stream, const DeviceState **out = nullptr)
+int ensure_ready(hipStream_t stream, const DeviceState **out)
 {
     int dev = 0;
     hipError_t e = hipGetDevice(&dev);
@@ -870,56 +839,4 @@ int dispatch_f16(const void *x, const void *codes, const void *grid, float scale
         return run_gemv_regx<false>(x, codes, grid, scale, y, M, N, K, s);
     if (gemm_ok(x, codes, grid, y, M, N, K)) return run_gemm(x, codes, grid, scale, y, M, N, K, s);
     return run_generic(x, codes, grid, scale, y, M, N, K, s);
-}
-
-// ------------------------------------------------------------------ the operator on host memory
-// The reference's own CPU path is a scalar decode and a triple loop (/root/reference/test_decode_matmul.py:29-71);
-// this is the same thing for the half-precision form, in plain C++ for tensors that live in host
-// memory: no GPU is involved and no GPU call is made.  Not a fallback: device pointers never come
-// here, the entry points below are separate ones.  One rounding per weight (the fp32 sum of a half
-// and +-1/4 is exact), fp32 sums over k in ascending order, rows of W spread over host threads.
-inline void host_decode_row(const uint16_t *codes, const half_t *grid, int64_t kc, half_t *w)
-{
-    for (int64_t j = 0; j < kc; j++) {
-        const uint32_t c = codes[j];
-        const uint32_t idx = c & 0xFFu, s7 = (c >> 8) & 0x7Fu;
-        const uint32_t s8 = s7 | ((uint32_t)(__builtin_popcount(s7) & 1) << 7);
-        const float shift = (c & 0x8000u) ? -0.25f : 0.25f;
-        for (int d = 0; d < 8; d++) {
-            const float g = (float)grid[idx * 8 + d];
-            w[j * 8 + d] = (half_t)(((s8 >> d) & 1u ? -g : g) + shift);
-        }
-    }
-}
-
-// Rows [0, n_rows) split over host threads; body(n0, n1) must not throw.  Threads cost about 50 us
-// each to start, so only work of 2^24 multiply-adds or more (several milliseconds on one core) gets
-// any, and never more than one per 2^22.  If a thread cannot be started the rows it was to
-// take run on the calling thread.
-template <typename F>
-void host_parallel_rows(int64_t n_rows, int64_t work_per_row, F body) noexcept
-{
-    const int64_t work = n_rows * work_per_row;
-    unsigned threads = std::thread::hardware_concurrency();
-    if (threads == 0) threads = 1;
-    if (threads > 16) threads = 16;
-    if ((int64_t)threads > (work >> 22)) threads = (unsigned)(work >> 22);
-    if ((int64_t)threads > n_rows) threads = (unsigned)n_rows;
-    if (work < (1 << 24) || threads < 2) {
-        body(0, n_rows);
-        return;
-    }
-    std::thread pool[16];
-    unsigned started = 0;
-    for (unsigned t = 1; t < threads; t++) {
-        try {
-            pool[started] = std::thread([=] { body(n_rows * t / threads, n_rows * (t + 1) / threads); });
-        } catch (...) {   // std::system_error: no more threads to be had
-            body(n_rows * t / threads, n_rows);
-            break;
-        }
-        started++;
-    }
-    body(0, n_rows / threads);
-    for (unsigned t = 0; t < started; t++) pool[t].join();
 }

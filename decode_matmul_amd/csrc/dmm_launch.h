@@ -1,0 +1,49 @@
+// What the two translation units of the library share on the host side: launch plumbing and the
+// per-device set-up (defined in dmm_host.h).
+// Part of libdmm: included by dmm.hip and dmm_ops.hip inside namespace dmm; not a translation unit of
+// its own.
+
+extern thread_local hipEvent_t tls_start;   // dmm_set_kernel_events
+extern thread_local hipEvent_t tls_stop;
+
+template <typename T>
+struct same_type { typedef T type; };
+
+// Enqueue one kernel; the status is what the launch call itself returns (no look at the
+// thread's last-error state, which may hold somebody else's stale error).  kFirst / kLast:
+// whether this launch opens / closes the span the timing events bracket (an operator call
+// that takes two kernels records start before the first and stop after the second).
+template <bool kFirst = true, bool kLast = true, typename... KArgs>
+int launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t shmem, hipStream_t stream,
+           typename same_type<KArgs>::type... args)
+{
+    void *argv[] = {(void *)&args...};
+    if (tls_start && tls_stop)
+        return (int)hipExtLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, argv, shmem, stream,
+                                       kFirst ? tls_start : nullptr, kLast ? tls_stop : nullptr, 0);
+    return (int)hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, argv, shmem, stream);
+}
+
+inline bool aligned(const void *p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+constexpr int kLdsMax = 160 * 1024;
+
+// Every kernel that needs more dynamic LDS than the default limit, or whose table addressing
+// assumes that its dynamic LDS starts at LDS address 0 (true exactly when the kernel has no
+// static LDS, which dmm_init verifies from the function's attributes).
+struct KernelInfo {
+    const void *fn;
+    int dynamic_lds;   // bytes to allow; 0 = default limit is enough
+    bool lds_base0;
+};
+
+template <typename... KArgs>
+KernelInfo kinfo(void (*k)(KArgs...), int lds, bool base0) { return KernelInfo{reinterpret_cast<const void *>(k), lds, base0}; }
+
+// the kernels of dmm_ops.hip, for dmm_init
+const std::vector<KernelInfo> &ops_kernel_table();
+
+struct DeviceState;
+int ensure_ready(hipStream_t stream, const DeviceState **out = nullptr);   // set-up of the current device on its first call
+int cu_count();              // compute units of the current device, after ensure_ready
+int cu_count_or_default();   // the same for pure queries: 256 before the device is set up

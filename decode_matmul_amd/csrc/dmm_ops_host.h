@@ -1,0 +1,204 @@
+// The host side of the operators around the product: checks, dispatch, and the same operators on host memory.
+// Part of libdmm: included by dmm_ops.hip inside namespace dmm; not a translation unit of its own.
+
+inline bool type_ok(int t) { return t == DMM_F16 || t == DMM_F32; }
+inline uintptr_t type_bytes(int t) { return t == DMM_F32 ? 4 : 2; }
+
+// what both products ask of their arguments; on_y: rows of y, codes: E matrices
+int check_ops(const void *x, int64_t T, const void *codes, const void *grid, const dmm_epilogue *ep, const void *y, int64_t R,
+              int64_t E, int64_t N, int64_t K)
+{
+    if (!ep) return DMM_ERR_NULL_POINTER;
+    if (T < 0 || R < 0 || E < 0 || N < 0 || K < 0 || (K & 7)) return DMM_ERR_BAD_SHAPE;
+    if (ep->activation < DMM_ACT_NONE || ep->activation > DMM_ACT_GELU_TANH || !type_ok(ep->out_type) ||
+        (ep->bias && !type_ok(ep->bias_type)) || (ep->residual && !type_ok(ep->residual_type)))
+        return DMM_ERR_BAD_SHAPE;
+    if (R == 0 || N == 0 || E == 0) return DMM_OK;
+    if (!y || !grid) return DMM_ERR_NULL_POINTER;
+    if (K > 0 && (!codes || (T > 0 && !x))) return DMM_ERR_NULL_POINTER;
+    if (!aligned(x, 2) || !aligned(codes, 2) || !aligned(grid, 2) || !aligned(y, type_bytes(ep->out_type)) ||
+        (ep->bias && !aligned(ep->bias, type_bytes(ep->bias_type))) ||
+        (ep->residual && !aligned(ep->residual, type_bytes(ep->residual_type))))
+        return DMM_ERR_MISALIGNED;
+    if (T > INT32_MAX || R > INT32_MAX || E > 65535 || N > INT32_MAX / 2 || K > INT32_MAX) return DMM_ERR_TOO_LARGE;
+    return DMM_OK;
+}
+
+Epi make_epi(const dmm_epilogue &ep, void *y, int64_t N, const float *scales, int scale_cols)
+{
+    Epi e;
+    e.bias = ep.bias;
+    e.residual = ep.residual;
+    e.y = y;
+    e.scales = scales;
+    e.scale = ep.scale;
+    e.scale_up = ep.scale_up;
+    e.N = (int)N;
+    e.act = ep.activation;
+    e.scale_cols = scale_cols;
+    e.bias_f32 = ep.bias_type == DMM_F32;
+    e.residual_f32 = ep.residual_type == DMM_F32;
+    e.out_f32 = ep.out_type == DMM_F32;
+    auto four = [](const void *p, int type) { return !p || aligned(p, 4 * type_bytes(type)); };
+    e.vec = (N & 3) == 0 && four(y, ep.out_type) && four(ep.bias, ep.bias_type) && four(ep.residual, ep.residual_type);
+    return e;
+}
+
+template <bool kGated>
+int run_ops_generic(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    int64_t blocks = ((int64_t)e.N + 3) / 4;
+    if (blocks > 65535 * 16) blocks = 65535 * 16;
+    return launch(ops_generic_kernel<kGated>, dim3((unsigned)blocks, (unsigned)g.E), dim3(256), 0, s, (const uint16_t *)x,
+                  (const uint16_t *)codes, grid, g, e, K);
+}
+
+int dispatch_ops(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, bool gated, int64_t K,
+                 hipStream_t s)
+{
+    return gated ? run_ops_generic<true>(x, codes, grid, g, e, K, s) : run_ops_generic<false>(x, codes, grid, g, e, K, s);
+}
+
+const std::vector<KernelInfo> &ops_kernel_table()
+{
+    static const std::vector<KernelInfo> t = {
+        kinfo(route_choose_kernel<1, false>, kLdsMax, false), kinfo(route_choose_kernel<2, false>, kLdsMax, false),
+        kinfo(route_choose_kernel<4, false>, kLdsMax, false), kinfo(route_choose_kernel<8, false>, kLdsMax, false),
+        kinfo(route_choose_kernel<16, false>, kLdsMax, false),
+    };
+    return t;
+}
+
+// ------------------------------------------------------------------ choice of experts
+// 64 tokens per block; more tokens take more words per expert's mask, so that the second kernel's sums over the
+// blocks stay short (512 blocks, up to eight words)
+inline int route_words(int64_t T)
+{
+    int w = 1;
+    while (w < 8 && T > (int64_t)w * 64 * 512) w *= 2;
+    return w;
+}
+inline int64_t route_blocks(int64_t T) { return (T + 64 * route_words(T) - 1) / (64 * route_words(T)); }
+
+template <int EV>
+int launch_route(const RouteArgs &a, int64_t blocks, hipStream_t s)
+{
+    const size_t masks = (size_t)a.E * a.words * 8;
+    if (blocks == 1)
+        return launch(route_choose_kernel<EV, true>, dim3(1), dim3(1024), masks + (size_t)(a.E + 1) * 4, s, a);
+    const int st = launch<true, false>(route_choose_kernel<EV, false>, dim3((unsigned)blocks), dim3(1024), masks, s, a);
+    if (st != 0) return st;
+    return launch<false, true>(route_place_kernel, dim3((unsigned)blocks), dim3(1024), (size_t)(3 * a.E + 1) * 4, s, a);
+}
+
+// ------------------------------------------------------------------ the operators on host memory
+// Plain loops, the same order of roundings as the device (sums in fp32, one rounding at the store).
+inline float host_load(const void *p, int64_t i, int type)
+{
+    if (type == DMM_F32) return reinterpret_cast<const float *>(p)[i];
+    if (type == DMM_BF16) {
+        const uint32_t u = (uint32_t)reinterpret_cast<const uint16_t *>(p)[i] << 16;
+        return __builtin_bit_cast(float, u);
+    }
+    return (float)reinterpret_cast<const half_t *>(p)[i];
+}
+
+inline void host_store(void *p, int64_t i, int type, float v)
+{
+    if (type == DMM_F32) reinterpret_cast<float *>(p)[i] = v;
+    else reinterpret_cast<half_t *>(p)[i] = (half_t)v;
+}
+
+inline float host_act(float z, int act)
+{
+    switch (act) {
+        case DMM_ACT_RELU: return z < 0.f ? 0.f : z;
+        case DMM_ACT_SILU: return z / (1.f + expf(-z));
+        case DMM_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752440f));
+        case DMM_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286535588f * (z + 0.044715f * z * z * z)));
+        default: return z;
+    }
+}
+
+int host_ops(const void *x, int64_t T, const int32_t *rows, const void *codes, const void *grid, const float *scales, int scale_cols,
+             const int32_t *offsets, const dmm_epilogue &ep, void *y, int64_t R, int64_t E, int64_t N, int64_t K)
+{
+    const int64_t kc = K >> 3, N2 = ep.gated ? 2 * N : N;
+    const half_t *xh = (const half_t *)x;
+    std::atomic<int> failed{0};
+    std::atomic<int> *failed_p = &failed;
+    for (int64_t e = 0; e < E; e++) {
+        int64_t lo = 0, hi = R;
+        if (offsets) {
+            lo = offsets[e] < 0 ? 0 : offsets[e] > R ? R : offsets[e];
+            hi = offsets[e + 1] < lo ? lo : offsets[e + 1] > R ? R : offsets[e + 1];
+        }
+        if (lo == hi) continue;
+        float s = ep.scale, su = ep.scale_up;
+        if (scales) {
+            s *= scales[e * scale_cols];
+            su *= scales[e * scale_cols + scale_cols - 1];
+        }
+        const uint16_t *ce = (const uint16_t *)codes + e * N2 * kc;
+        host_parallel_rows(N, 2 * K * (hi - lo + 1), [=, &ep](int64_t n0, int64_t n1) {
+            half_t *w = (half_t *)malloc((size_t)(2 * K + 1) * sizeof(half_t));   // a decoded row, and its partner
+            if (!w) {
+                failed_p->store(1, std::memory_order_relaxed);
+                return;
+            }
+            for (int64_t n = n0; n < n1; n++) {
+                host_decode_row(ce + n * kc, (const half_t *)grid, kc, w);
+                if (ep.gated) host_decode_row(ce + (N + n) * kc, (const half_t *)grid, kc, w + K);
+                for (int64_t p = lo; p < hi; p++) {
+                    const int64_t t = rows ? rows[p] : p;
+                    float v = 0.f, u = 0.f;
+                    if (t >= 0 && t < T) {
+                        for (int64_t k = 0; k < K; k++) v += (float)xh[t * K + k] * (float)w[k];
+                        if (ep.gated)
+                            for (int64_t k = 0; k < K; k++) u += (float)xh[t * K + k] * (float)w[K + k];
+                    }
+                    float z = v * s;
+                    if (ep.bias) z += host_load(ep.bias, e * N2 + n, ep.bias_type);
+                    z = host_act(z, ep.activation);
+                    if (ep.gated) {
+                        float zu = u * su;
+                        if (ep.bias) zu += host_load(ep.bias, e * N2 + N + n, ep.bias_type);
+                        z *= zu;
+                    }
+                    if (ep.residual) z += host_load(ep.residual, p * N + n, ep.residual_type);
+                    host_store(y, p * N + n, ep.out_type, z);
+                }
+            }
+            free(w);
+        });
+    }
+    return failed.load(std::memory_order_relaxed) ? DMM_ERR_HOST_MEMORY : DMM_OK;
+}
+
+int check_route(const void *logits, int type, int64_t T, int64_t E, int64_t k, int scoring, const void *weights, const void *experts,
+                const void *offsets, const void *rows, const void *slots)
+{
+    if (T < 0 || E < 1 || k < 1 || k > E) return DMM_ERR_BAD_SHAPE;
+    if (type != DMM_F16 && type != DMM_F32 && type != DMM_BF16) return DMM_ERR_BAD_SHAPE;
+    if (scoring != DMM_SCORE_SOFTMAX && scoring != DMM_SCORE_SIGMOID) return DMM_ERR_BAD_SHAPE;
+    if (E > kRouteMaxE || k > kRouteMaxK || T * k > INT32_MAX) return DMM_ERR_TOO_LARGE;
+    if (!offsets || (T > 0 && (!logits || !weights || !experts || !rows || !slots))) return DMM_ERR_NULL_POINTER;
+    if (!aligned(logits, type_bytes(type)) || !aligned(weights, 4) || !aligned(experts, 4) || !aligned(offsets, 4) || !aligned(rows, 4) ||
+        !aligned(slots, 4))
+        return DMM_ERR_MISALIGNED;
+    return DMM_OK;
+}
+
+int check_combine(const void *y, int y_type, const void *slots, const void *weights, const void *residual, int residual_type,
+                  const void *out, int out_type, int64_t R, int64_t T, int64_t k, int64_t N)
+{
+    if (R < 0 || T < 0 || k < 0 || N < 0) return DMM_ERR_BAD_SHAPE;
+    if (!type_ok(y_type) || !type_ok(out_type) || (residual && !type_ok(residual_type))) return DMM_ERR_BAD_SHAPE;
+    if (T == 0 || N == 0) return DMM_OK;
+    if (!out || (k > 0 && (!slots || !weights)) || (k > 0 && R > 0 && !y)) return DMM_ERR_NULL_POINTER;
+    if (!aligned(y, type_bytes(y_type)) || !aligned(slots, 4) || !aligned(weights, 4) || !aligned(out, type_bytes(out_type)) ||
+        (residual && !aligned(residual, type_bytes(residual_type))))
+        return DMM_ERR_MISALIGNED;
+    if (R > INT32_MAX || T > INT32_MAX || k > INT32_MAX || N > INT32_MAX - 4096) return DMM_ERR_TOO_LARGE;
+    return DMM_OK;
+}

@@ -1,5 +1,6 @@
 // PyTorch-ROCm operator over the C ABI of libdmm.so.  Host code only: no device code is
-// compiled here, the kernels live in dmm.hip and the dmm_*.h files it includes, behind include/dmm.h.
+// compiled here, the kernels live in dmm.hip, dmm_ops.hip and the dmm_*.h files they include, behind
+// include/dmm.h.
 //
 // Mirrors the operator boundary of the reference,
 // /root/reference/decode_matmul_cuda/decode_matmul_cuda.cu:178-239: one module, a function
@@ -237,6 +238,263 @@ torch::Tensor decode_matmul_int8(torch::Tensor x, torch::Tensor weights_compress
     return out;
 }
 
+// ------------------------------------------------------------------ the operators around the product
+// All tensors of a call are on one device: a GPU, or the host, whose tensors take the library's host
+// route.  The weights are frozen codes and no operator here has a gradient: an input that asks for one is refused.
+typedef c10::optional<torch::Tensor> MaybeTensor;
+
+#define DMM_CHECK_SAME_DEVICE(t, dev) TORCH_CHECK((t).device() == (dev), #t " must be on ", (dev), " like x")
+
+void check_no_grad(const torch::Tensor &t, const char *what, const char *name)
+{
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, ": ", name,
+                " requires a gradient, which this operator does not compute; call it under torch.no_grad() or detach the input");
+}
+
+void check_device(const torch::Device &d, const char *what)
+{
+    TORCH_CHECK(d.is_cuda() || d.is_cpu(), what, ": tensors must be on a GPU or on the host");
+}
+
+int float_type(const torch::Tensor &t, const char *name)
+{
+    if (t.scalar_type() == torch::kHalf) return DMM_F16;
+    TORCH_CHECK(t.scalar_type() == torch::kFloat, name, " must be float16 or float32");
+    return DMM_F32;
+}
+
+int out_type_of(torch::ScalarType t)
+{
+    TORCH_CHECK(t == torch::kHalf || t == torch::kFloat, "out_dtype must be float16 or float32");
+    return t == torch::kHalf ? DMM_F16 : DMM_F32;
+}
+
+int activation_of(const std::string &name)
+{
+    if (name == "none") return DMM_ACT_NONE;
+    if (name == "relu") return DMM_ACT_RELU;
+    if (name == "silu") return DMM_ACT_SILU;
+    if (name == "gelu") return DMM_ACT_GELU;
+    if (name == "gelu_tanh") return DMM_ACT_GELU_TANH;
+    TORCH_CHECK(false, "unknown activation '", name, "' (none, relu, silu, gelu, gelu_tanh)");
+}
+
+hipStream_t stream_of(const torch::Device &d)
+{
+    return d.is_cuda() ? c10::hip::getCurrentHIPStream(d.index()).stream() : nullptr;
+}
+
+// the code matrix (or matrices) and the grid, on x's device
+void check_weights(const torch::Tensor &x, const torch::Tensor &codes, const torch::Tensor &grid, int64_t dim, const char *what)
+{
+    check_device(x.device(), what);
+    DMM_CHECK_CONTIGUOUS(x);
+    DMM_CHECK_CONTIGUOUS(codes);
+    DMM_CHECK_CONTIGUOUS(grid);
+    DMM_CHECK_SAME_DEVICE(codes, x.device());
+    DMM_CHECK_SAME_DEVICE(grid, x.device());
+    TORCH_CHECK(x.scalar_type() == torch::kHalf, "x must be float16");
+    TORCH_CHECK(x.dim() == 2, "x must be [rows, K]");
+    TORCH_CHECK(is_code_dtype(codes), "codes must be int16 or uint16");
+    TORCH_CHECK(codes.dim() == dim, dim == 2 ? "codes must be [N, K/8]" : "codes must be [E, N, K/8]");
+    TORCH_CHECK(grid.scalar_type() == torch::kHalf && grid.dim() == 2 && grid.size(0) == 256 && grid.size(1) == 8,
+                "grid must be float16 [256, 8]");
+    TORCH_CHECK(x.size(1) == codes.size(-1) * 8, "x.size(-1) must be 8 * codes.size(-1)");
+    check_no_grad(x, what, "x");
+    check_no_grad(grid, what, "grid");
+}
+
+torch::Tensor decode_matmul_fused(torch::Tensor x, torch::Tensor codes, torch::Tensor grid, double scale, double scale_up,
+                                  MaybeTensor bias, const std::string &activation, bool gated, MaybeTensor residual,
+                                  torch::ScalarType out_dtype)
+{
+    check_weights(x, codes, grid, 2, "decode_matmul_fused");
+    const int64_t M = x.size(0), K = x.size(1), rows = codes.size(0);
+    TORCH_CHECK(!gated || rows % 2 == 0, "a gated call needs the gate's rows and as many up rows in codes");
+    const int64_t N = gated ? rows / 2 : rows;
+    dmm_epilogue ep{};
+    ep.activation = activation_of(activation);
+    ep.gated = gated;
+    ep.scale = static_cast<float>(scale);
+    ep.scale_up = static_cast<float>(scale_up);
+    ep.out_type = out_type_of(out_dtype);
+    if (bias) {
+        DMM_CHECK_SAME_DEVICE(*bias, x.device());
+        DMM_CHECK_CONTIGUOUS(*bias);
+        TORCH_CHECK(bias->dim() == 1 && bias->size(0) == rows, "bias must have one value per row of codes");
+        check_no_grad(*bias, "decode_matmul_fused", "bias");
+        ep.bias_type = float_type(*bias, "bias");
+        ep.bias = bias->data_ptr();
+    }
+    if (residual) {
+        DMM_CHECK_SAME_DEVICE(*residual, x.device());
+        DMM_CHECK_CONTIGUOUS(*residual);
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == M && residual->size(1) == N, "residual must be [M, N]");
+        check_no_grad(*residual, "decode_matmul_fused", "residual");
+        ep.residual_type = float_type(*residual, "residual");
+        ep.residual = residual->data_ptr();
+    }
+    c10::OptionalDeviceGuard guard;
+    if (x.is_cuda()) guard.reset_device(x.device());
+    torch::Tensor y = torch::empty({M, N}, x.options().dtype(out_dtype).requires_grad(false));
+    torch::Tensor workspace;
+    const int64_t ws_bytes = x.is_cuda() ? dmm_fused_workspace_bytes(M, N, K, gated) : 0;
+    if (ws_bytes > 0) workspace = torch::empty({ws_bytes}, x.options().dtype(torch::kUInt8).requires_grad(false));
+    hipStream_t stream = stream_of(x.device());
+    int st;
+    {
+        pybind11::gil_scoped_release nogil;
+        st = x.is_cpu() ? dmm_decode_matmul_fused_host(x.data_ptr(), codes.data_ptr(), grid.data_ptr(), &ep, y.data_ptr(), M, N, K)
+                        : dmm_decode_matmul_fused(x.data_ptr(), codes.data_ptr(), grid.data_ptr(), &ep, y.data_ptr(), M, N, K,
+                                                  ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, stream);
+    }
+    check_status(st, "decode_matmul_fused");
+    return y;
+}
+
+torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch::Tensor grid, double scale, MaybeTensor scales,
+                                    torch::Tensor offsets, MaybeTensor rows, MaybeTensor bias, const std::string &activation,
+                                    bool gated, torch::ScalarType out_dtype, MaybeTensor out)
+{
+    check_weights(x, codes, grid, 3, "decode_matmul_grouped");
+    const int64_t T = x.size(0), K = x.size(1), E = codes.size(0), wrows = codes.size(1);
+    TORCH_CHECK(!gated || wrows % 2 == 0, "a gated call needs the gate's rows and as many up rows in codes");
+    const int64_t N = gated ? wrows / 2 : wrows;
+    DMM_CHECK_SAME_DEVICE(offsets, x.device());
+    DMM_CHECK_CONTIGUOUS(offsets);
+    TORCH_CHECK(offsets.scalar_type() == torch::kInt32 && offsets.dim() == 1 && offsets.size(0) == E + 1,
+                "offsets must be int32 with one more entry than codes has experts");
+    int64_t R = T;
+    if (rows) {
+        DMM_CHECK_SAME_DEVICE(*rows, x.device());
+        DMM_CHECK_CONTIGUOUS(*rows);
+        TORCH_CHECK(rows->scalar_type() == torch::kInt32 && rows->dim() == 1, "rows must be int32 [R]");
+        R = rows->size(0);
+    }
+    dmm_epilogue ep{};
+    ep.activation = activation_of(activation);
+    ep.gated = gated;
+    ep.scale = ep.scale_up = static_cast<float>(scale);
+    ep.out_type = out_type_of(out_dtype);
+    int scale_cols = 1;
+    if (scales) {
+        DMM_CHECK_SAME_DEVICE(*scales, x.device());
+        DMM_CHECK_CONTIGUOUS(*scales);
+        TORCH_CHECK(scales->scalar_type() == torch::kFloat && scales->size(0) == E &&
+                        (scales->dim() == 1 || (gated && scales->dim() == 2 && scales->size(1) == 2)),
+                    "scale must be a number, float32 [E], or float32 [E, 2] for a gated call");
+        check_no_grad(*scales, "decode_matmul_grouped", "scale");
+        scale_cols = static_cast<int>(scales->dim());
+    }
+    if (bias) {
+        DMM_CHECK_SAME_DEVICE(*bias, x.device());
+        DMM_CHECK_CONTIGUOUS(*bias);
+        TORCH_CHECK(bias->dim() == 2 && bias->size(0) == E && bias->size(1) == wrows, "bias must have one value per row of codes");
+        check_no_grad(*bias, "decode_matmul_grouped", "bias");
+        ep.bias_type = float_type(*bias, "bias");
+        ep.bias = bias->data_ptr();
+    }
+    c10::OptionalDeviceGuard guard;
+    if (x.is_cuda()) guard.reset_device(x.device());
+    torch::Tensor y;
+    if (out) {
+        DMM_CHECK_SAME_DEVICE(*out, x.device());
+        DMM_CHECK_CONTIGUOUS(*out);
+        TORCH_CHECK(out->dim() == 2 && out->size(0) == R && out->size(1) == N && out->scalar_type() == out_dtype,
+                    "out must be [R, N] of out_dtype");
+        check_no_grad(*out, "decode_matmul_grouped", "out");
+        y = *out;
+    } else {
+        y = torch::empty({R, N}, x.options().dtype(out_dtype).requires_grad(false));
+    }
+    hipStream_t stream = stream_of(x.device());
+    const void *rp = rows ? rows->data_ptr() : nullptr, *sp = scales ? scales->data_ptr() : nullptr;
+    int st;
+    {
+        pybind11::gil_scoped_release nogil;
+        st = x.is_cpu() ? dmm_decode_matmul_grouped_host(x.data_ptr(), T, rp, codes.data_ptr(), grid.data_ptr(), sp, scale_cols,
+                                                         offsets.data_ptr(), &ep, y.data_ptr(), R, E, N, K)
+                        : dmm_decode_matmul_grouped(x.data_ptr(), T, rp, codes.data_ptr(), grid.data_ptr(), sp, scale_cols,
+                                                    offsets.data_ptr(), &ep, y.data_ptr(), R, E, N, K, stream);
+    }
+    check_status(st, "decode_matmul_grouped");
+    return y;
+}
+
+std::vector<torch::Tensor> route_experts(torch::Tensor logits, int64_t k, const std::string &scoring, bool normalize)
+{
+    check_device(logits.device(), "route_experts");
+    DMM_CHECK_CONTIGUOUS(logits);
+    TORCH_CHECK(logits.dim() == 2, "logits must be [T, E]");
+    TORCH_CHECK(scoring == "softmax" || scoring == "sigmoid", "unknown scoring '", scoring, "' (softmax, sigmoid)");
+    check_no_grad(logits, "route_experts", "logits");
+    const int type = logits.scalar_type() == torch::kBFloat16 ? DMM_BF16 : float_type(logits, "logits must be bfloat16, or");
+    const int64_t T = logits.size(0), E = logits.size(1);
+    TORCH_CHECK(k >= 1 && k <= E && k <= 64 && E <= 1024, "k must be between 1 and min(E, 64), and E at most 1024");
+    const int sc = scoring == "sigmoid" ? DMM_SCORE_SIGMOID : DMM_SCORE_SOFTMAX;
+    c10::OptionalDeviceGuard guard;
+    if (logits.is_cuda()) guard.reset_device(logits.device());
+    const auto i32 = logits.options().dtype(torch::kInt32).requires_grad(false);
+    torch::Tensor weights = torch::empty({T, k}, i32.dtype(torch::kFloat)), experts = torch::empty({T, k}, i32),
+                  offsets = torch::empty({E + 1}, i32), rows = torch::empty({T * k}, i32), slots = torch::empty({T, k}, i32);
+    torch::Tensor workspace;
+    const int64_t ws_bytes = logits.is_cuda() ? dmm_route_workspace_bytes(T, E) : 0;
+    if (ws_bytes > 0) workspace = torch::empty({ws_bytes}, i32.dtype(torch::kUInt8));
+    hipStream_t stream = stream_of(logits.device());
+    int st;
+    {
+        pybind11::gil_scoped_release nogil;
+        st = logits.is_cpu() ? dmm_route_experts_host(logits.data_ptr(), type, T, E, k, sc, normalize, weights.data_ptr(),
+                                                      experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr())
+                             : dmm_route_experts(logits.data_ptr(), type, T, E, k, sc, normalize, weights.data_ptr(), experts.data_ptr(),
+                                                 offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
+                                                 ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, stream);
+    }
+    check_status(st, "route_experts");
+    return {weights, experts, offsets, rows, slots};
+}
+
+torch::Tensor combine_experts(torch::Tensor y, torch::Tensor slots, torch::Tensor weights, MaybeTensor residual,
+                              torch::ScalarType out_dtype)
+{
+    check_device(y.device(), "combine_experts");
+    DMM_CHECK_CONTIGUOUS(y);
+    DMM_CHECK_CONTIGUOUS(slots);
+    DMM_CHECK_CONTIGUOUS(weights);
+    TORCH_CHECK(slots.device() == y.device() && weights.device() == y.device(), "y, slots and weights must be on the same device");
+    TORCH_CHECK(y.dim() == 2, "y must be [R, N]");
+    TORCH_CHECK(slots.scalar_type() == torch::kInt32 && slots.dim() == 2, "slots must be int32 [T, k]");
+    TORCH_CHECK(weights.scalar_type() == torch::kFloat && weights.sizes() == slots.sizes(), "weights must be float32 [T, k]");
+    check_no_grad(y, "combine_experts", "y");
+    check_no_grad(weights, "combine_experts", "weights");
+    const int y_type = float_type(y, "y"), out_type = out_type_of(out_dtype);
+    const int64_t R = y.size(0), N = y.size(1), T = slots.size(0), k = slots.size(1);
+    const void *rp = nullptr;
+    int r_type = DMM_F16;
+    if (residual) {
+        TORCH_CHECK(residual->device() == y.device(), "residual must be on the same device as y");
+        DMM_CHECK_CONTIGUOUS(*residual);
+        TORCH_CHECK(residual->dim() == 2 && residual->size(0) == T && residual->size(1) == N, "residual must be [T, N]");
+        check_no_grad(*residual, "combine_experts", "residual");
+        r_type = float_type(*residual, "residual");
+        rp = residual->data_ptr();
+    }
+    c10::OptionalDeviceGuard guard;
+    if (y.is_cuda()) guard.reset_device(y.device());
+    torch::Tensor out = torch::empty({T, N}, y.options().dtype(out_dtype).requires_grad(false));
+    hipStream_t stream = stream_of(y.device());
+    int st;
+    {
+        pybind11::gil_scoped_release nogil;
+        st = y.is_cpu() ? dmm_combine_experts_host(y.data_ptr(), y_type, slots.data_ptr(), weights.data_ptr(), rp, r_type, out.data_ptr(),
+                                                   out_type, R, T, k, N)
+                        : dmm_combine_experts(y.data_ptr(), y_type, slots.data_ptr(), weights.data_ptr(), rp, r_type, out.data_ptr(),
+                                              out_type, R, T, k, N, stream);
+    }
+    check_status(st, "combine_experts");
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
@@ -255,4 +513,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("x"), pybind11::arg("packed"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("N"));
     m.def("decode", &decode, "Decode codes [N, K/8] to the dense half matrix [N, K]",
           pybind11::arg("codes"), pybind11::arg("grid"));
+    m.def("decode_matmul_fused", &decode_matmul_fused, "decode_matmul with bias, activation, gate and residual in its epilogue",
+          pybind11::arg("x"), pybind11::arg("codes"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("scale_up"),
+          pybind11::arg("bias"), pybind11::arg("activation"), pybind11::arg("gated"), pybind11::arg("residual"),
+          pybind11::arg("out_dtype"));
+    m.def("decode_matmul_grouped", &decode_matmul_grouped, "decode_matmul_fused per expert, rows grouped by expert",
+          pybind11::arg("x"), pybind11::arg("codes"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("scales"),
+          pybind11::arg("offsets"), pybind11::arg("rows"), pybind11::arg("bias"), pybind11::arg("activation"), pybind11::arg("gated"),
+          pybind11::arg("out_dtype"), pybind11::arg("out"));
+    m.def("route_experts", &route_experts, "The k largest logits per row, their weights, and the rows sorted by expert",
+          pybind11::arg("logits"), pybind11::arg("k"), pybind11::arg("scoring"), pybind11::arg("normalize"));
+    m.def("combine_experts", &combine_experts, "Weighted sum of the experts' rows", pybind11::arg("y"), pybind11::arg("slots"),
+          pybind11::arg("weights"), pybind11::arg("residual"), pybind11::arg("out_dtype"));
 }

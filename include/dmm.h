@@ -277,6 +277,93 @@ int dmm_decode_host_f16(const void *codes, const void *grid, void *W, int64_t N,
 int dmm_decode_matmul_host_f16(const void *x, const void *codes, const void *grid, float scale,
                                void *y, int64_t M, int64_t N, int64_t K);
 
+/* ---- the operators around the product ------------------------------------------------------------
+ * None has a counterpart in the reference, whose one operator is the bare product.  All of them enqueue
+ * on the caller's stream, allocate nothing, never synchronise, and can be captured (after dmm_init).
+ * Results do not depend on how workgroups are scheduled: no floating-point atomics. */
+
+/* element types */
+enum { DMM_F16 = 0, DMM_F32 = 1, DMM_BF16 = 2 };
+/* activations: z; max(z, 0); z / (1 + exp(-z)); z Phi(z) with erf; the same with tanh:
+ * z / 2 (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) */
+enum { DMM_ACT_NONE = 0, DMM_ACT_RELU = 1, DMM_ACT_SILU = 2, DMM_ACT_GELU = 3, DMM_ACT_GELU_TANH = 4 };
+
+/* What is done to a finished sum, in fp32 with one rounding at the store:
+ *   z = scale * sum + bias;   y = act(z)                          gated == 0: W has N rows
+ *   y = act(z[n]) * z[N + n]                                      gated != 0: W has 2 N rows, gate then up
+ *   y += residual
+ * Types are DMM_F16 or DMM_F32; a NULL bias or residual is left out and its type not looked at. */
+typedef struct dmm_epilogue {
+    const void *bias;        /* [N], gated [2 N] (grouped: one such row per expert)       */
+    const void *residual;    /* [M, N]; may be y itself.  dmm_decode_matmul_grouped: NULL  */
+    int32_t bias_type, residual_type, out_type;
+    int32_t activation;      /* DMM_ACT_...                                               */
+    int32_t gated;
+    float scale;             /* of the rows 0 .. N - 1 of W                               */
+    float scale_up;          /* of the rows N .. 2 N - 1, gated calls only                */
+} dmm_epilogue;
+
+/* The product with an epilogue: y[M,N] from x half [M,K], codes [N,K/8] (gated: [2 N,K/8]), grid half [256,8], as
+ * dmm_decode_matmul_f16 takes them; K % 8 == 0 is the only shape demand, K == 0 is an empty sum.  K % 16 == 0
+ * with 16-byte aligned x, codes and grid runs on the matrix unit, everything else on the catch-all.
+ * The workspace is that of dmm_decode_matmul_ws_f16: dmm_fused_workspace_bytes bytes let a short x split K as far
+ * as it would like, fewer (or NULL, 0) only limit the split. */
+int64_t dmm_fused_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated);
+int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, const dmm_epilogue *epilogue,
+                            void *y, int64_t M, int64_t N, int64_t K, void *workspace,
+                            int64_t workspace_bytes, void *stream);
+
+/* The product grouped by expert, ragged: row p of y [R,N] for offsets[e] <= p < offsets[e + 1] is made with expert e's
+ * matrix, codes [E,N,K/8] (gated: [E,2 N,K/8]), from row rows[p] of x half [T,K].
+ *   offsets  int32 [E + 1] on the device, not decreasing, from 0 to at most R: the sizes need not be known
+ *            on the host.  Broken lists are cut to 0 <= first <= last <= R, never followed out of a buffer.
+ *   rows     int32 [R] on the device, or NULL: row p itself (then T == R).  An entry outside 0 .. T - 1
+ *            stands for a row of zeros.
+ *   scales   float [E] on the device, times the epilogue's scale and scale_up; scale_cols == 2 (gated only):
+ *            [E,2], gate and up; or NULL.
+ * Rows of y that belong to no expert (from offsets[E] on) are left as they were.  Up to 65535 experts. */
+int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const void *codes, const void *grid,
+                              const void *scales, int scale_cols, const void *offsets,
+                              const dmm_epilogue *epilogue, void *y, int64_t R, int64_t E, int64_t N, int64_t K,
+                              void *stream);
+
+/* The choice of experts: for every row of logits [T,E] (half, bfloat16 or float) the k largest, largest first, equal ones
+ * by index; a logit of -inf (or NaN) is never chosen, so a row may have fewer than k choices or none.
+ *   weights  float [T,k]: softmax over the row (DMM_SCORE_SOFTMAX) or 1 / (1 + exp(-v)) (DMM_SCORE_SIGMOID) of the
+ *            chosen, divided by their sum if normalize; 0 for a choice that was not made.  A NaN in a
+ *            row makes its weights NaN.
+ *   experts  int32 [T,k], -1 for a choice that was not made
+ *   offsets  int32 [E + 1]: first row of every expert when the choices are sorted by expert, then by token
+ *   rows     int32 [T * k]: the token of every sorted row, -1 from offsets[E] on; what
+ *            dmm_decode_matmul_grouped takes
+ *   slots    int32 [T,k]: the sorted row of every choice, -1 for one that was not made; what
+ *            dmm_combine_experts takes
+ * E <= 1024, k <= min(E, 64).  The workspace (16-byte aligned, dmm_route_workspace_bytes, 0 up to 64 tokens) is needed
+ * whole: fewer bytes are refused with DMM_ERR_SCRATCH_TOO_SMALL. */
+enum { DMM_SCORE_SOFTMAX = 0, DMM_SCORE_SIGMOID = 1 };
+int64_t dmm_route_workspace_bytes(int64_t T, int64_t E);
+int dmm_route_experts(const void *logits, int logits_type, int64_t T, int64_t E, int64_t k, int scoring, int normalize,
+                      void *weights, void *experts, void *offsets, void *rows, void *slots, void *workspace,
+                      int64_t workspace_bytes, void *stream);
+
+/* The weighted sum of the experts' rows: out[t] = residual[t] + sum over j, in order, of weights[t,j] * y[slots[t,j]], in fp32
+ * with one rounding; y [R,N] and out [T,N] half or float, weights float [T,k], slots int32 [T,k].  A slot outside
+ * 0 .. R - 1 adds nothing.  residual [T,N] half or float, or NULL; it may be out itself. */
+int dmm_combine_experts(const void *y, int y_type, const void *slots, const void *weights, const void *residual,
+                        int residual_type, void *out, int out_type, int64_t R, int64_t T, int64_t k, int64_t N,
+                        void *stream);
+
+/* The four on host memory (every pointer a host pointer), blocking, as dmm_decode_matmul_host_f16. */
+int dmm_decode_matmul_fused_host(const void *x, const void *codes, const void *grid, const dmm_epilogue *epilogue,
+                                 void *y, int64_t M, int64_t N, int64_t K);
+int dmm_decode_matmul_grouped_host(const void *x, int64_t T, const void *rows, const void *codes, const void *grid,
+                                   const void *scales, int scale_cols, const void *offsets,
+                                   const dmm_epilogue *epilogue, void *y, int64_t R, int64_t E, int64_t N, int64_t K);
+int dmm_route_experts_host(const void *logits, int logits_type, int64_t T, int64_t E, int64_t k, int scoring,
+                           int normalize, void *weights, void *experts, void *offsets, void *rows, void *slots);
+int dmm_combine_experts_host(const void *y, int y_type, const void *slots, const void *weights, const void *residual,
+                             int residual_type, void *out, int out_type, int64_t R, int64_t T, int64_t k, int64_t N);
+
 /* Yardstick for benchmarks: a kernel that only READS a row-major code matrix [N, K/8] with the
  * batch-1 kernels' launch shape and access pattern (16 rows x 64 bytes per wave load) and does no
  * decoding; timed with dmm_set_kernel_events like any other call, it shows what the memory system
