@@ -269,12 +269,19 @@ __host__ __device__ constexpr int gr_smem_bytes(int TM) { return kSTablesBytes +
 // shorter x.  kSplit: blockIdx.z picks a contiguous share of the k tiles and the block writes
 // fp32 partial sums to part[z][M][N] instead of y (summed, scaled and rounded by
 // splitk_reduce_kernel), so that short x still fills the chip with workgroups.
-template <int TM, bool kSplit, bool kPacked>
-__global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restrict__ x,
-                                                       const uint16_t *__restrict__ codes,
-                                                       const void *__restrict__ grid, float scale,
-                                                       uint16_t *__restrict__ y, float *__restrict__ part,
-                                                       int M, int N, int K, int splits, int y_vec)
+//
+// The body serves the operators of dmm_ops.hip too.  What differs is the place P: which rows of y, x and W a
+// workgroup has, whether the last k tile may be cut (kRagged), and what becomes of the sums.
+//   p.m0, p.m_end           first row of y of the block, end of the rows it may touch
+//   p.x_base(m)             byte offset of the row of x behind row m of y; kGrOut: none (zeros)
+//   p.w_row(i, wave, l32)   row of W for lane l32 of row tile i of a wave; -1: none
+//   p.finish(acc, ...)      the sums: acc[i][j], D layout below
+constexpr int kGrOut = (int)0x80000000;   // an offset no buffer reaches
+
+template <int TM, bool kSplit, bool kPacked, class P>
+__device__ __forceinline__ void gemm_reg_body(const P &p, const uint16_t *__restrict__ x, int64_t x_bytes,
+                                              const uint16_t *__restrict__ codes, int N, const void *__restrict__ grid, int K,
+                                              int splits)
 {
     constexpr int kBM = 32 * TM;
     extern __shared__ __attribute__((aligned(256))) unsigned char smem_raw[];
@@ -286,12 +293,11 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
     const uint32_t quarter_bits = 0x34003400u;
     // Workgroups go to the 8 XCDs round robin by linear id, so with m fastest the workgroups
     // of one XCD share a few x row blocks (which then stay in that XCD's L2) and stream the codes.
-    const int m0 = blockIdx.x * kBM;
-    const int n0 = blockIdx.y * kGrBN;
+    const int m0 = p.m0;
     const int row_bytes = K >> 2;
-    constexpr int kOut = (int)0x80000000;
+    constexpr int kOut = kGrOut;
     // this block's k tiles: [kt_lo, kt_lo + k_tiles)
-    int kt_lo = 0, k_tiles = K / kGrBK;
+    int kt_lo = 0, k_tiles = P::kRagged ? (K + kGrBK - 1) / kGrBK : K / kGrBK;
     if (kSplit) {
         const int z = blockIdx.z, tq = k_tiles / splits, tr = k_tiles % splits;
         kt_lo = z * tq + (z < tr ? z : tr);
@@ -321,7 +327,7 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
     const __amdgpu_buffer_rsrc_t crsrc = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t *>(codes), 0, (int)((int64_t)(kPacked ? n_pad : N) * row_bytes), 0x00020000);
     const __amdgpu_buffer_rsrc_t xrsrc =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(x), 0, (int)((int64_t)M * K * 2), 0x00020000);
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(x), 0, (int)x_bytes, 0x00020000);
     // Row-major codes travel four k tiles at a time: lane (row, half kq) loads the 32 bytes of its row that
     // hold tiles 4 j + 2 kq and 4 j + 2 kq + 1 whole, so the two lanes of a row take 64 consecutive bytes
     // (half a cache line per visit, not 16 bytes of it), and one v_permlane32_swap per word hands lanes
@@ -331,18 +337,19 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
     int cvoff[kGrTN];
 #pragma unroll
     for (int i = 0; i < kGrTN; i++) {
-        const int n = n0 + wave * 64 + i * 32 + l32;
+        const int n = p.w_row(i, wave, l32);
         if (kPacked) cvoff[i] = n < n_pad ? (n >> 4) * (K >> 8) * 1024 + (n & 15) * 16 + kq * 8 : kOut;
-        else cvoff[i] = n < N ? n * row_bytes + kq * 32 : kOut;
+        else cvoff[i] = (uint32_t)n < (uint32_t)N ? n * row_bytes + kq * 32 : kOut;
     }
     // rows r and r + 8 share a group of 16 lanes: with the 144-byte pitch their 16 pieces fall in
     // 16 different bank groups, so the LDS writes below are conflict-free like the fragment reads
     const int x_row = ((tid >> 7) << 4) + ((tid >> 4) & 7) + (((tid >> 3) & 1) << 3), x_piece = tid & 7;
     int xvoff[TM];
 #pragma unroll
-    for (int p = 0; p < TM; p++) {
-        const int m = m0 + 32 * p + x_row;
-        xvoff[p] = m < M ? (m * K + x_piece * 8) * 2 : kOut;
+    for (int j = 0; j < TM; j++) {
+        const int m = m0 + 32 * j + x_row;
+        const int xb = m < p.m_end ? p.x_base(m, K) : kOut;
+        xvoff[j] = xb != kOut ? xb + x_piece * 16 : kOut;
     }
 
     struct Stage {
@@ -378,9 +385,11 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
                     ct.w[i][h][w + 2] = r[1];
                 }
     };
-    auto load_x = [&](Stage &st, int kt, int p) {
+    auto load_x = [&](Stage &st, int kt, int j) {
         const int xoff = kt < k_tiles ? (kt_lo + kt) * 128 : kOut;
-        st.xv[p] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, xvoff[p], xoff, 0);
+        // a cut last tile: the pieces past K belong to the next row of x, zeros in their place
+        const int xv = P::kRagged && (kt_lo + kt) * kGrBK + x_piece * 8 >= K ? kOut : xvoff[j];
+        st.xv[j] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, xv, xoff, 0);
     };
     auto load_tile = [&](Stage &st, int kt) {
         if constexpr (!kWide) load_codes(st, kt);
@@ -534,44 +543,72 @@ __global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restric
     if (kt + 1 < k_tiles) tile(kt + 1, 1, ring[2], ring[1], N2{});
     if (kt + 2 < k_tiles) tile(kt + 2, 0, ring[3], ring[2], N3{});
 
-    // D layout of 32x32: element e of lane: row (n) = 8*(e/4) + 4*(lane/32) + e%4, column (m) = lane%32
-    const bool n_vec = (N & 3) == 0 && (kSplit || y_vec != 0);   // 8-byte stores need an 8-byte aligned y
+    p.template finish<TM>(acc, wave, l32, kq, tid, smem_raw);
+}
+
+// The plain product: rows and columns by block index.
+template <bool kSplit>
+struct GemmPlainPlace {
+    static constexpr bool kRagged = false;
+    int m0, m_end, n0, N, y_vec;
+    float scale;
+    uint16_t *y;
+    float *part;
+    __device__ __forceinline__ int x_base(int m, int K) const { return m * K * 2; }
+    __device__ __forceinline__ int w_row(int i, int wave, int l32) const { return n0 + wave * 64 + i * 32 + l32; }
+    template <int TM>
+    __device__ __forceinline__ void finish(const f16_t (&acc)[kGrTN][TM], int wave, int l32, int kq, int, unsigned char *) const
+    {
+        // D layout of 32x32: element e of lane: row (n) = 8*(e/4) + 4*(lane/32) + e%4, column (m) = lane%32
+        const bool n_vec = (N & 3) == 0 && (kSplit || y_vec != 0);   // 8-byte stores need an 8-byte aligned y
 #pragma unroll
-    for (int i = 0; i < kGrTN; i++)
+        for (int i = 0; i < kGrTN; i++)
 #pragma unroll
-        for (int j = 0; j < TM; j++) {
-            const int m = m0 + j * 32 + l32;
-            if (m >= M) continue;
+            for (int j = 0; j < TM; j++) {
+                const int m = m0 + j * 32 + l32;
+                if (m >= m_end) continue;
 #pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                const int n = n0 + wave * 64 + i * 32 + 8 * e4 + 4 * kq;
-                if (kSplit) {
-                    float *dst = part + ((int64_t)blockIdx.z * M + m) * N + n;
+                for (int e4 = 0; e4 < 4; e4++) {
+                    const int n = n0 + wave * 64 + i * 32 + 8 * e4 + 4 * kq;
+                    if (kSplit) {
+                        float *dst = part + ((int64_t)blockIdx.z * m_end + m) * N + n;
+                        if (n_vec && n + 3 < N) {
+                            *reinterpret_cast<f4_t *>(dst) =
+                                f4_t{acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; e++)
+                                if (n + e < N) dst[e] = acc[i][j][4 * e4 + e];
+                        }
+                        continue;
+                    }
+                    uint16_t o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[e] = __builtin_bit_cast(uint16_t, (half_t)(acc[i][j][4 * e4 + e] * scale));
+                    uint16_t *dst = y + (int64_t)m * N + n;
                     if (n_vec && n + 3 < N) {
-                        *reinterpret_cast<f4_t *>(dst) =
-                            f4_t{acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
+                        u2_t v;
+                        v[0] = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
+                        v[1] = (uint32_t)o[2] | ((uint32_t)o[3] << 16);
+                        *reinterpret_cast<u2_t *>(dst) = v;
                     } else {
 #pragma unroll
                         for (int e = 0; e < 4; e++)
-                            if (n + e < N) dst[e] = acc[i][j][4 * e4 + e];
+                            if (n + e < N) dst[e] = o[e];
                     }
-                    continue;
-                }
-                uint16_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    o[e] = __builtin_bit_cast(uint16_t, (half_t)(acc[i][j][4 * e4 + e] * scale));
-                uint16_t *dst = y + (int64_t)m * N + n;
-                if (n_vec && n + 3 < N) {
-                    u2_t v;
-                    v[0] = (uint32_t)o[0] | ((uint32_t)o[1] << 16);
-                    v[1] = (uint32_t)o[2] | ((uint32_t)o[3] << 16);
-                    *reinterpret_cast<u2_t *>(dst) = v;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (n + e < N) dst[e] = o[e];
                 }
             }
-        }
+    }
+};
+
+template <int TM, bool kSplit, bool kPacked>
+__global__ __launch_bounds__(256) void gemm_reg_kernel(const uint16_t *__restrict__ x,
+                                                       const uint16_t *__restrict__ codes,
+                                                       const void *__restrict__ grid, float scale,
+                                                       uint16_t *__restrict__ y, float *__restrict__ part,
+                                                       int M, int N, int K, int splits, int y_vec)
+{
+    const GemmPlainPlace<kSplit> p{(int)blockIdx.x * 32 * TM, M, (int)blockIdx.y * kGrBN, N, y_vec, scale, y, part};
+    gemm_reg_body<TM, kSplit, kPacked>(p, x, (int64_t)M * K * 2, codes, N, grid, K, splits);
 }

@@ -525,7 +525,7 @@ int launch_gemm_reg_tm(const void *x, const void *codes, const void *grid, float
 }
 
 // rows of x per block: 32, 64 or 128
-inline int gemm_reg_tm(int64_t M) { return M <= 32 ? 1 : M <= 64 ? 2 : 4; }
+int gemm_reg_tm(int64_t M) { return M <= 32 ? 1 : M <= 64 ? 2 : 4; }
 
 template <bool kPacked = false>
 int launch_gemm_reg(const void *x, const void *codes, const void *grid, float scale, void *y, int64_t M,
@@ -554,17 +554,30 @@ int splitk_plan(int64_t M, int64_t N, int64_t K, int64_t workspace_bytes, int cu
     return splits < 2 ? 1 : (int)splits;
 }
 
+// the first half of a split call: partial sums
+template <bool kPacked>
+int launch_gemm_parts(const void *x, const void *codes, const void *grid, float *part, int splits, int64_t M, int64_t N, int64_t K,
+                      hipStream_t stream)
+{
+    switch (gemm_reg_tm(M)) {
+        case 1: return launch_gemm_reg_tm<1, true, kPacked>(x, codes, grid, 1.f, nullptr, part, M, N, K, splits, stream);
+        case 2: return launch_gemm_reg_tm<2, true, kPacked>(x, codes, grid, 1.f, nullptr, part, M, N, K, splits, stream);
+        default: return launch_gemm_reg_tm<4, true, kPacked>(x, codes, grid, 1.f, nullptr, part, M, N, K, splits, stream);
+    }
+}
+
+int launch_gemm_partial(const void *x, const void *codes, const void *grid, float *part, int splits, int64_t M, int64_t N, int64_t K,
+                        hipStream_t stream)
+{
+    return launch_gemm_parts<false>(x, codes, grid, part, splits, M, N, K, stream);
+}
+
 template <bool kPacked = false>
 int launch_gemm_splitk(const void *x, const void *codes, const void *grid, float scale, void *y, void *workspace,
                        int splits, int64_t M, int64_t N, int64_t K, hipStream_t stream)
 {
     float *part = reinterpret_cast<float *>(workspace);
-    int st;
-    switch (gemm_reg_tm(M)) {
-        case 1: st = launch_gemm_reg_tm<1, true, kPacked>(x, codes, grid, scale, y, part, M, N, K, splits, stream); break;
-        case 2: st = launch_gemm_reg_tm<2, true, kPacked>(x, codes, grid, scale, y, part, M, N, K, splits, stream); break;
-        default: st = launch_gemm_reg_tm<4, true, kPacked>(x, codes, grid, scale, y, part, M, N, K, splits, stream); break;
-    }
+    const int st = launch_gemm_parts<kPacked>(x, codes, grid, part, splits, M, N, K, stream);
     if (st != 0) return st;
     const int64_t mn = M * N;
     const int64_t blocks = (mn + 1023) / 1024;
@@ -577,10 +590,6 @@ bool gemm_reg_ok(int64_t M, int64_t N, int64_t K)
 {
     return N * (K >> 2) < (1LL << 31) && M * K * 2 < (1LL << 31) && N <= 65535LL * kGrBN;
 }
-
-// Smallest M that takes the split-K path when a workspace is given (up to M = 16 the
-// matrix-vector kernels are as fast or faster).
-constexpr int kSplitKMinM = 17;
 
 // What passes of the small-batch kernel cost, us: 2 for the launch, the code bytes once at 5.5 TB/s on 256
 // compute units (the first pass reads them from HBM), and per 16 rows of x about 0.9, the code bytes at

@@ -47,3 +47,12 @@ struct DeviceState;
 int ensure_ready(hipStream_t stream, const DeviceState **out = nullptr);   // set-up of the current device on its first call
 int cu_count();              // compute units of the current device, after ensure_ready
 int cu_count_or_default();   // the same for pure queries: 256 before the device is set up
+
+// the plain product's split of K, which the product with an epilogue shares: the plan, and the kernel that leaves
+// fp32 partial sums in part [splits][M][N]
+constexpr int kSplitKMinM = 17;   // smallest M that splits (up to M = 16 the matrix-vector kernels are as fast or faster)
+int gemm_reg_tm(int64_t M);       // rows of x per block / 32
+bool gemm_reg_ok(int64_t M, int64_t N, int64_t K);
+int splitk_plan(int64_t M, int64_t N, int64_t K, int64_t workspace_bytes, int cus);
+int launch_gemm_partial(const void *x, const void *codes, const void *grid, float *part, int splits, int64_t M, int64_t N, int64_t K,
+                        hipStream_t stream);

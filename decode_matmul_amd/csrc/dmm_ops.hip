@@ -23,7 +23,10 @@ namespace dmm {
 #include "dmm_launch.h"
 #include "dmm_hostroute.h"
 #include "dmm_tables.h"
+#include "dmm_gemv_f16.h"
+#include "dmm_gemm.h"
 #include "dmm_epilogue.h"
+#include "dmm_ops_gemm.h"
 #include "dmm_route.h"
 #include "dmm_ops_host.h"
 
@@ -42,10 +45,11 @@ int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, 
     if (workspace && workspace_bytes > 0 && !aligned(workspace, 16)) return DMM_ERR_MISALIGNED;
     if ((st = ensure_ready((hipStream_t)stream))) return st;
     const Groups g{nullptr, nullptr, 1, (int)M, (int)M};
-    return dispatch_ops(x, codes, grid, g, make_epi(*ep, y, N, nullptr, 1), ep->gated != 0, K, (hipStream_t)stream);
+    return dispatch_ops(x, codes, grid, g, make_epi(*ep, y, N, nullptr, 1), ep->gated != 0, K, workspace, workspace_bytes,
+                        (hipStream_t)stream);
 }
 
-int64_t dmm_fused_workspace_bytes(int64_t, int64_t, int64_t, int) { return 0; }
+int64_t dmm_fused_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated) { return ops_workspace_bytes(M, N, K, gated != 0); }
 
 static int check_grouped(const void *x, int64_t T, const void *rows, const void *codes, const void *grid, const void *scales,
                          int scale_cols, const void *offsets, const dmm_epilogue *ep, const void *y, int64_t R, int64_t E, int64_t N,
@@ -68,7 +72,8 @@ int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const 
     if (st != DMM_OK || R == 0 || N == 0 || E == 0) return st;
     if ((st = ensure_ready((hipStream_t)stream))) return st;
     const Groups g{(const int32_t *)offsets, (const int32_t *)rows, (int)E, (int)R, (int)T};
-    return dispatch_ops(x, codes, grid, g, make_epi(*ep, y, N, (const float *)scales, scale_cols), ep->gated != 0, K, (hipStream_t)stream);
+    return dispatch_ops(x, codes, grid, g, make_epi(*ep, y, N, (const float *)scales, scale_cols), ep->gated != 0, K, nullptr, 0,
+                        (hipStream_t)stream);
 }
 
 int64_t dmm_route_workspace_bytes(int64_t T, int64_t E)

@@ -53,18 +53,79 @@ int run_ops_generic(const void *x, const void *codes, const void *grid, const Gr
                   (const uint16_t *)codes, grid, g, e, K);
 }
 
-int dispatch_ops(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, bool gated, int64_t K,
-                 hipStream_t s)
+// the matrix unit's kernels: 16-byte loads at 4-byte aligned places, 31-bit offsets into x and one expert's codes
+bool ops_mfma_ok(const void *x, const void *codes, const void *grid, const Groups &g, int64_t rows, int64_t K)
 {
-    return gated ? run_ops_generic<true>(x, codes, grid, g, e, K, s) : run_ops_generic<false>(x, codes, grid, g, e, K, s);
+    return K >= 16 && (K & 15) == 0 && aligned(x, 16) && aligned(codes, 16) && aligned(grid, 16) && g.T > 0 &&
+           (int64_t)g.T * K * 2 < (1LL << 31) && rows * (K >> 2) < (1LL << 31) && rows <= 65535LL * 128;
+}
+
+template <int TM, bool kGated>
+int launch_ops_gemm(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    constexpr int BM = 32 * TM, BN = GemmOpsPlace<kGated>::kOutN;
+    const int64_t tiles = ((int64_t)g.R + BM - 1) / BM + (g.offsets ? g.E : 0);   // an expert adds at most one cut tile
+    return launch(ops_gemm_kernel<TM, kGated>, dim3((unsigned)tiles, (unsigned)((e.N + BN - 1) / BN)), dim3(256), gr_smem_bytes(TM), s,
+                  (const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K);
+}
+
+// rows of y per block by the rows an expert has on average
+template <bool kGated>
+int run_ops_gemm(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    switch (gemm_reg_tm(g.R / g.E)) {
+        case 1: return launch_ops_gemm<1, kGated>(x, codes, grid, g, e, K, s);
+        case 2: return launch_ops_gemm<2, kGated>(x, codes, grid, g, e, K, s);
+        default: return launch_ops_gemm<4, kGated>(x, codes, grid, g, e, K, s);
+    }
+}
+
+template <bool kGated>
+int run_ops(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, void *workspace,
+            int64_t workspace_bytes, hipStream_t s)
+{
+    const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
+    if (!ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
+    if (!g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 && gemm_reg_ok(g.R, rows, K)) {
+        const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cu_count());
+        if (splits >= 2) {
+            const int st = launch_gemm_partial(x, codes, grid, (float *)workspace, splits, g.R, rows, K, s);
+            if (st != 0) return st;
+            const int64_t cells = (int64_t)g.R * ((e.N + 3) / 4);
+            return launch<false, true>(ops_splitk_kernel<kGated>, dim3((unsigned)((cells + 255) / 256)), dim3(256), 0, s,
+                                       (const float *)workspace, e, g.R, splits);
+        }
+    }
+    return run_ops_gemm<kGated>(x, codes, grid, g, e, K, s);
+}
+
+int dispatch_ops(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, bool gated, int64_t K,
+                 void *workspace, int64_t workspace_bytes, hipStream_t s)
+{
+    return gated ? run_ops<true>(x, codes, grid, g, e, K, workspace, workspace_bytes, s)
+                 : run_ops<false>(x, codes, grid, g, e, K, workspace, workspace_bytes, s);
+}
+
+// 0: no split
+int64_t ops_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated)
+{
+    const int64_t rows = gated ? 2 * N : N;
+    if (M < kSplitKMinM || N < 1 || K < 64 || (K & 63) || M > 65535LL * 128 || !gemm_reg_ok(M, rows, K)) return 0;
+    const int splits = splitk_plan(M, rows, K, INT64_MAX, cu_count_or_default());
+    return splits >= 2 ? (int64_t)splits * M * rows * 4 : 0;
 }
 
 const std::vector<KernelInfo> &ops_kernel_table()
 {
     static const std::vector<KernelInfo> t = {
-        kinfo(route_choose_kernel<1, false>, kLdsMax, false), kinfo(route_choose_kernel<2, false>, kLdsMax, false),
-        kinfo(route_choose_kernel<4, false>, kLdsMax, false), kinfo(route_choose_kernel<8, false>, kLdsMax, false),
-        kinfo(route_choose_kernel<16, false>, kLdsMax, false),
+#define DMM_K_OPS(G)                                                                                                     \
+    kinfo(ops_gemm_kernel<1, G>, gr_smem_bytes(1), true), kinfo(ops_gemm_kernel<2, G>, gr_smem_bytes(2), true),         \
+        kinfo(ops_gemm_kernel<4, G>, gr_smem_bytes(4), true)
+        DMM_K_OPS(false), DMM_K_OPS(true),
+#undef DMM_K_OPS
+#define DMM_K_ROUTE(EV) kinfo(route_choose_kernel<EV, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, true>, kLdsMax, false)
+        DMM_K_ROUTE(1), DMM_K_ROUTE(2), DMM_K_ROUTE(4), DMM_K_ROUTE(8), DMM_K_ROUTE(16),
+#undef DMM_K_ROUTE
     };
     return t;
 }
