@@ -56,6 +56,7 @@ _GROUPED = [_P, _I64, _P, _P, _P, _P, _INT, _P, _EP, _P, _I64, _I64, _I64, _I64]
 _ROUTE = [_P, _INT, _I64, _I64, _I64, _INT, _INT, _P, _P, _P, _P, _P]
 _COMBINE = [_P, _INT, _P, _P, _P, _INT, _P, _INT, _I64, _I64, _I64, _I64]
 SYMBOLS.update({
+    "dmm_set_ops_kernel": (_INT, [_INT]),
     "dmm_fused_workspace_bytes": (_I64, [_I64, _I64, _I64, _INT]),
     "dmm_decode_matmul_fused": (_INT, [_P, _P, _P, _EP, _P, _I64, _I64, _I64, _P, _I64, _P]),
     "dmm_decode_matmul_fused_host": (_INT, [_P, _P, _P, _EP, _P, _I64, _I64, _I64]),

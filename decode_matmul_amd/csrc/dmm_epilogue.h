@@ -47,9 +47,16 @@ __device__ __forceinline__ float epi_load(const void *p, int64_t i, int f32)
     return f32 ? reinterpret_cast<const float *>(p)[i] : (float)reinterpret_cast<const half_t *>(p)[i];
 }
 
-// four elements from i on, i % 4 == 0 (N % 4 == 0, see Epi::vec)
-__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32)
+// four elements from i on, one by one (the first `left` of them) unless vec: i % 4 == 0 and p aligned, see Epi::vec
+__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32, int vec, int left)
 {
+    if (!vec) {
+        f4_t r = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < left) r[k] = epi_load(p, i + k, f32);
+        return r;
+    }
     if (f32) return *reinterpret_cast<const f4_t *>(reinterpret_cast<const float *>(p) + i);
     const h4_t h = *reinterpret_cast<const h4_t *>(reinterpret_cast<const half_t *>(p) + i);
     return f4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
@@ -87,31 +94,49 @@ __device__ __forceinline__ void epi_store1(const Epi &e, const EpiScale &sc, flo
     else reinterpret_cast<half_t *>(e.y)[i] = (half_t)z;
 }
 
+// The activation of four values.  kSmall: one after the other in a loop (the vector turned by one element each
+// time), a quarter of the code and of the registers, for kernels that have none to spare; else side by side, which
+// hides the latency where few waves run.
+template <bool kSmall>
+__device__ __forceinline__ f4_t epi_act4(f4_t z, int act)
+{
+    if constexpr (kSmall) {
+        if (act == DMM_ACT_NONE) return z;
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) z = f4_t{z[1], z[2], z[3], epi_act(z[0], act)};
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) z[i] = epi_act(z[i], act);
+    }
+    return z;
+}
+
 // four outputs (row, n .. n + 3), n % 4 == 0; those past N are left out
-template <bool kGated>
+template <bool kGated, bool kSmall>
 __device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n,
                                            int expert)
 {
-    if (!e.vec) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (n + i < e.N) epi_store1<kGated>(e, sc, v[i], u[i], row, n + i, expert);
-        return;
-    }
     if (n >= e.N) return;
+    const int left = e.N - n;   // outputs that exist, from here on
     const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
     f4_t z = v * sc.s;
-    if (e.bias) z += epi_load4(e.bias, b, e.bias_f32);
-#pragma unroll
-    for (int i = 0; i < 4; i++) z[i] = epi_act(z[i], e.act);
+    if (e.bias) z += epi_load4(e.bias, b, e.bias_f32, e.vec, left);
+    z = epi_act4<kSmall>(z, e.act);
     if (kGated) {
         f4_t w = u * sc.up;
-        if (e.bias) w += epi_load4(e.bias, b + e.N, e.bias_f32);
+        if (e.bias) w += epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
         z *= w;
     }
     const int64_t i = row * e.N + n;
-    if (e.residual) z += epi_load4(e.residual, i, e.residual_f32);
-    if (e.out_f32) {
+    if (e.residual) z += epi_load4(e.residual, i, e.residual_f32, e.vec, left);
+    if (!e.vec) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (k >= left) break;
+            if (e.out_f32) reinterpret_cast<float *>(e.y)[i + k] = z[k];
+            else reinterpret_cast<half_t *>(e.y)[i + k] = (half_t)z[k];
+        }
+    } else if (e.out_f32) {
         *reinterpret_cast<f4_t *>(reinterpret_cast<float *>(e.y) + i) = z;
     } else {
         h4_t o;

@@ -6,6 +6,7 @@
 // Kernels and host code in the files included below, each inside namespace dmm; the decode tables, the
 // matrix-vector helpers and the matrix-matrix kernel's body are shared with dmm.hip.
 #include <hip/hip_runtime.h>
+#include <algorithm>
 #include <atomic>
 #include <thread>
 #include <type_traits>
@@ -24,8 +25,10 @@ namespace dmm {
 #include "dmm_hostroute.h"
 #include "dmm_tables.h"
 #include "dmm_gemv_f16.h"
+#include "dmm_gemv_f16d.h"
 #include "dmm_gemm.h"
 #include "dmm_epilogue.h"
+#include "dmm_ops_rows.h"
 #include "dmm_ops_gemm.h"
 #include "dmm_route.h"
 #include "dmm_ops_host.h"
@@ -47,6 +50,12 @@ int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, 
     const Groups g{nullptr, nullptr, 1, (int)M, (int)M};
     return dispatch_ops(x, codes, grid, g, make_epi(*ep, y, N, nullptr, 1), ep->gated != 0, K, workspace, workspace_bytes,
                         (hipStream_t)stream);
+}
+
+int dmm_set_ops_kernel(int kernel)
+{
+    if (kernel < -1 || kernel > kOpsSplit) return DMM_ERR_BAD_SHAPE;
+    return g_ops_kernel.exchange(kernel, std::memory_order_relaxed);
 }
 
 int64_t dmm_fused_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated) { return ops_workspace_bytes(M, N, K, gated != 0); }

@@ -57,7 +57,7 @@ struct GemmOpsPlace {
             const float *src = tile + r * kPitch + c;
             const f4_t v = *reinterpret_cast<const f4_t *>(src);
             const f4_t u = kGated ? *reinterpret_cast<const f4_t *>(src + kOutN) : f4_t{0.f, 0.f, 0.f, 0.f};
-            epi_store4<kGated>(epi, sc, v, u, m0 + r, n, expert);
+            epi_store4<kGated, false>(epi, sc, v, u, m0 + r, n, expert);
         }
     }
 };
@@ -130,5 +130,5 @@ __global__ __launch_bounds__(256) void ops_splitk_kernel(const float *__restrict
                     if (kGated) u[k] += src[z * plane + epi.N + k];
                 }
     }
-    epi_store4<kGated>(epi, epi_scale(epi, 0), v, u, m, n, 0);
+    epi_store4<kGated, false>(epi, epi_scale(epi, 0), v, u, m, n, 0);
 }

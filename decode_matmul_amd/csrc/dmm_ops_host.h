@@ -80,13 +80,58 @@ int run_ops_gemm(const void *x, const void *codes, const void *grid, const Group
     }
 }
 
+// dmm_set_ops_kernel: what a test or a benchmark forces instead of the choice below (-1: nothing)
+std::atomic<int> g_ops_kernel{-1};
+enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3 };
+
+template <int NT, int XI, int W, int CG, bool kGated>
+int launch_ops_rows_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
+                         hipStream_t s)
+{
+    const int64_t wgs = units < cu_count() ? units : cu_count();
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K};
+    return launch(ops_rows_kernel<NT, 2, XI, W, CG, kGated>, dim3((unsigned)wgs), dim3(64 * W), (size_t)fd_lds_bytes(XI, W), s, args);
+}
+
+// most segments the rows can make, sr rows each: an expert adds at most one cut one, and none without a row
+inline int64_t ops_segments(const Groups &g, int64_t sr)
+{
+    const int64_t full = ((int64_t)g.R + sr - 1) / sr;
+    return g.offsets ? std::min<int64_t>((int64_t)g.R, (int64_t)g.R / sr + g.E) : full;
+}
+
+template <int XI, int W, int CG, bool kGated>
+int launch_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t units = ops_segments(g, 2 * XI * CG) * ((e.N + 15) / 16);
+    const int64_t cus = cu_count(), share = (units + cus - 1) / cus * (kGated ? 2 : 1);   // most tiles a workgroup gets
+    if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
+    if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
+    return launch_ops_rows_inst<8, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
+}
+
+// rows of a segment by the rows an expert has
+template <bool kGated>
+int run_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t rows = g.offsets ? std::min<int64_t>(g.R, 2 * (int64_t)g.R / g.E + 2) : g.R;
+    if (rows <= 4) return launch_ops_rows<2, 16, 1, kGated>(x, codes, grid, g, e, K, s);
+    if (rows <= 8) return launch_ops_rows<4, 16, 1, kGated>(x, codes, grid, g, e, K, s);
+    if (rows <= 16) return launch_ops_rows<8, 8, 1, kGated>(x, codes, grid, g, e, K, s);
+    return launch_ops_rows<8, 8, 2, kGated>(x, codes, grid, g, e, K, s);
+}
+
 template <bool kGated>
 int run_ops(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, void *workspace,
             int64_t workspace_bytes, hipStream_t s)
 {
     const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
-    if (!ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
-    if (!g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 && gemm_reg_ok(g.R, rows, K)) {
+    const int force = g_ops_kernel.load(std::memory_order_relaxed);
+    if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
+    const bool rows_ok = ops_segments(g, 4) * ((e.N + 15) / 16) < (1LL << 31);
+    if (rows_ok && (force == kOpsRows || (force < 0 && g.R / g.E <= 32))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    if (force != kOpsGemm && !g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 &&
+        gemm_reg_ok(g.R, rows, K)) {
         const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cu_count());
         if (splits >= 2) {
             const int st = launch_gemm_partial(x, codes, grid, (float *)workspace, splits, g.R, rows, K, s);
@@ -123,6 +168,13 @@ const std::vector<KernelInfo> &ops_kernel_table()
         kinfo(ops_gemm_kernel<4, G>, gr_smem_bytes(4), true)
         DMM_K_OPS(false), DMM_K_OPS(true),
 #undef DMM_K_OPS
+#define DMM_K_ROWS_X(NT, G)                                                                                             \
+    kinfo(ops_rows_kernel<NT, 2, 2, 16, 1, G>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 4, 16, 1, G>, kLdsMax, true), \
+        kinfo(ops_rows_kernel<NT, 2, 8, 8, 1, G>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 8, 8, 2, G>, kLdsMax, true)
+#define DMM_K_ROWS(G) DMM_K_ROWS_X(2, G), DMM_K_ROWS_X(4, G), DMM_K_ROWS_X(8, G)
+        DMM_K_ROWS(false), DMM_K_ROWS(true),
+#undef DMM_K_ROWS
+#undef DMM_K_ROWS_X
 #define DMM_K_ROUTE(EV) kinfo(route_choose_kernel<EV, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, true>, kLdsMax, false)
         DMM_K_ROUTE(1), DMM_K_ROUTE(2), DMM_K_ROUTE(4), DMM_K_ROUTE(8), DMM_K_ROUTE(16),
 #undef DMM_K_ROUTE

@@ -1,0 +1,329 @@
+// Few rows of x per matrix: the product with an epilogue and the product by expert on 16-bit operands.
+// Part of libdmm: included by dmm_ops.hip inside namespace dmm; not a translation unit of its own.
+
+// ------------------------------------------------------------------ the work, cut into jobs
+// A segment is up to SR rows of y of one expert (a dense call is one expert); a unit is a segment times 16 columns of
+// y: one 16-row tile of W, or for a gated call two, the gate's and the up projection's.  All units are numbered,
+// segment by segment, and dealt out as contiguous ranges that differ by at most one unit, one range per
+// workgroup and one workgroup per compute unit, whatever the experts' sizes are: an expert with many rows simply has more
+// segments, and the workgroups that walk its other segments at the same time find its codes in the caches.  A
+// workgroup goes through its range in jobs of up to NU units of one segment.
+//
+// A job is what gemv_f16d_kernel does: chunk of k steps outside, one step per wave; the slice of x of the step
+// through the wave's own piece of LDS into eight B operands; tiles inside, every tile's accumulator in registers; code
+// loads in a ring of D per wave, which here runs on into the next job (and so do the loads of x).  At the end of a
+// job the partial sums go through the pieces, a thread adds up four outputs over the waves in order and runs the
+// epilogue on them.
+// LDS map: tables [0, 96K), then W pieces of XI KB.
+struct OpsCursor {
+    int expert, row, row_end;   // segment: rows row .. of an expert whose rows end at row_end
+    int unit, left;             // next unit inside the segment, units left in the range
+    int per;                    // units per job in this segment
+};
+
+typedef __attribute__((address_space(4))) const int32_t const_i32_t;
+
+// an element of a list that no kernel writes meanwhile, at the same place in all lanes: through the scalar cache
+__device__ __forceinline__ int uniform_load(const int32_t *p, int i)
+{
+    return reinterpret_cast<const_i32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+}
+
+__device__ __forceinline__ GroupRange uniform_range(const Groups &g, int e)
+{
+    const int a = uniform_load(g.offsets, e), b = uniform_load(g.offsets, e + 1);
+    GroupRange r;
+    r.lo = a < 0 ? 0 : a > g.R ? g.R : a;
+    r.hi = b < r.lo ? r.lo : b > g.R ? g.R : b;
+    return r;
+}
+
+// inclusive sum over the lanes of a wave
+__device__ __forceinline__ int wave_scan(int v, int lane)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(v, off, kWave);
+        if (lane >= off) v += o;
+    }
+    return v;
+}
+
+__device__ __forceinline__ int cut_up(const GroupRange &r, int by) { return (int)(((uint32_t)(r.hi - r.lo) + (uint32_t)by - 1u) / (uint32_t)by); }
+
+// the units per job for `n` units of a segment: as few jobs as possible, of even size
+template <int NU>
+__device__ __forceinline__ int per_job(int n)
+{
+    const int jobs = (n + NU - 1) / NU;
+    return jobs <= 1 ? n : (n + jobs - 1) / jobs;
+}
+
+// the workgroup's range of units; false: it has none
+template <int SR, int NU>
+__device__ __forceinline__ bool ops_range(const Groups &g, int upn, int lane, OpsCursor &c)
+{
+    int segs, first_scan = 0;
+    GroupRange first{0, 0};
+    if (!g.offsets) {
+        segs = (g.R + SR - 1) / SR;
+    } else {
+        if (lane < g.E) first = group_range(g, lane);
+        first_scan = wave_scan(cut_up(first, SR), lane);
+        segs = __builtin_amdgcn_readlane(first_scan, 63);
+        for (int e0 = 64; e0 < g.E; e0 += 64) {
+            GroupRange r{0, 0};
+            if (e0 + lane < g.E) r = group_range(g, e0 + lane);
+            segs += __builtin_amdgcn_readlane(wave_scan(cut_up(r, SR), lane), 63);
+        }
+    }
+    const uint32_t units = (uint32_t)segs * (uint32_t)upn;   // below 2^31 (the host's business)
+    const uint32_t u0 = (uint32_t)((uint64_t)units * blockIdx.x / gridDim.x), u1 = (uint32_t)((uint64_t)units * (blockIdx.x + 1) / gridDim.x);
+    if (u0 >= u1) return false;
+    const int seg = (int)(u0 / (uint32_t)upn);
+    c.unit = (int)(u0 - (uint32_t)seg * (uint32_t)upn);
+    c.left = (int)(u1 - u0);
+    if (!g.offsets) {
+        c.expert = 0;
+        c.row = seg * SR;
+        c.row_end = g.R;
+    } else {
+        int base = 0;
+        for (int e0 = 0;; e0 += 64) {   // seg < segs: found
+            GroupRange r = first;
+            int s = first_scan;
+            if (e0 > 0) {
+                r = GroupRange{0, 0};
+                if (e0 + lane < g.E) r = group_range(g, e0 + lane);
+                s = wave_scan(cut_up(r, SR), lane);
+            }
+            const uint64_t here = __builtin_amdgcn_ballot_w64(seg < base + s);
+            if (here != 0 || e0 + 64 >= g.E) {
+                const int l = here != 0 ? __builtin_ctzll(here) : 0;
+                const int before = base + __builtin_amdgcn_readlane(s - cut_up(r, SR), l);
+                c.expert = e0 + l;
+                c.row = __builtin_amdgcn_readlane(r.lo, l) + (seg - before) * SR;
+                c.row_end = __builtin_amdgcn_readlane(r.hi, l);
+                break;
+            }
+            base += __builtin_amdgcn_readlane(s, 63);
+        }
+    }
+    const int in_seg = c.left < upn - c.unit ? c.left : upn - c.unit;
+    c.per = per_job<NU>(in_seg);
+    return true;
+}
+
+// a job's share of a chunk; n == 0: nothing
+struct OpsItem {
+    int expert, row, row_end, unit, n, chunk;
+};
+
+// The kernel's one argument, so that its address in the constant kernel-argument segment is known.  What is needed
+// once per job (the epilogue) is read from there when it is needed, not held in scalar registers through the loop.
+struct OpsRowsArgs {
+    const uint16_t *x, *codes;
+    const void *grid;
+    Groups g;
+    Epi epi;
+    int K;
+};
+typedef __attribute__((address_space(4))) const OpsRowsArgs const_rows_args_t;
+
+__device__ __forceinline__ const_rows_args_t *rows_args_late()
+{
+    uint64_t p = (uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));   // a value of its own: loads through it stay where they are written
+    return reinterpret_cast<const_rows_args_t *>((uintptr_t)p);
+}
+
+// XI, W, CG as in gemv_f16d_kernel: 2 XI rows of x per group, W waves, CG groups of sixteen rows per segment.
+template <int NT, int D, int XI, int W, int CG, bool kGated>
+__global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
+{
+    const uint16_t *__restrict__ x = args.x;
+    const uint16_t *__restrict__ codes = args.codes;
+    const Groups g = args.g;
+    const int K = args.K, N = args.epi.N;
+    constexpr int CM = 2 * XI;
+    constexpr int SR = CG * CM;          // rows of a segment
+    constexpr int kPiece = XI * 1024;
+    constexpr int NU = kGated ? NT / 2 : NT;
+    static_assert((W == 16 && (XI == 2 || XI == 4)) || (W == 8 && XI == 8), "up to four, eight or sixteen rows of x");
+    static_assert(CG == 1 || (CG == 2 && XI == 8), "a second group of rows only beside a full first one");
+    static_assert(fd_lds_bytes(XI, W) <= 160 * 1024, "tables and pieces have to fit the LDS");
+    static_assert(NT % D == 0 && (!kGated || NT % 2 == 0), "the ring has to divide the tiles");
+    static_assert(NT * 4 * CM * 16 <= kPiece, "the partial sums of a job go through the wave's piece");
+    constexpr bool kAhead = W == 8 ? !(NT == 8 && CG == 2) : NT < (XI == 4 && kGated ? 4 : 8);   // a code word's gathers ahead of the word before it, where registers are left
+    extern __shared__ __attribute__((aligned(256))) unsigned char smem_raw[];
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c16 = lane & 15;
+    const int q = lane >> 4;
+    const int n_steps = (K + 255) >> 8;
+    const int n_chunks = (n_steps + W - 1) / W;
+    const int row_bytes = K >> 2;
+    const int w_rows = kGated ? 2 * N : N;
+    const int upn = (N + 15) >> 4;
+    const uint32_t lane_base = (uint32_t)c16 * 16u;
+    const uint32_t quarter_bits = 0x34003400u;
+    constexpr int kOut = (int)0x80000000;
+
+    const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
+    OpsCursor cur;
+    if (!ops_range<SR, NU>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
+
+    // the next job, and the cursor behind it
+    auto next_job = [&]() {
+        OpsItem it{cur.expert, cur.row, cur.row_end, cur.unit, 0, 0};
+        if (cur.left == 0) return it;
+        const int in_seg = cur.left < upn - cur.unit ? cur.left : upn - cur.unit;
+        it.n = cur.per < in_seg ? cur.per : in_seg;
+        it.row_end = cur.row + SR < cur.row_end ? cur.row + SR : cur.row_end;
+        cur.left -= it.n;
+        cur.unit += it.n;
+        if (cur.unit == upn && cur.left > 0) {   // on to the next segment
+            cur.unit = 0;
+            cur.row += SR;
+            if (cur.row >= cur.row_end && g.offsets) {
+                GroupRange r{0, 0};
+                while (r.lo == r.hi && cur.expert + 1 < g.E) r = uniform_range(g, ++cur.expert);
+                cur.row = r.lo;
+                cur.row_end = r.hi;
+            }
+            cur.per = per_job<NU>(cur.left < upn ? cur.left : upn);
+        }
+        return it;
+    };
+    auto next_item = [&](const OpsItem &it) {
+        OpsItem o = it;
+        if (it.n > 0 && it.chunk + 1 < n_chunks) o.chunk++;
+        else o = next_job();
+        return o;
+    };
+
+    const __amdgpu_buffer_rsrc_t xrsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(x), 0, (int)((int64_t)g.T * K * 2), 0x00020000);
+    auto x_base = [&](int m, int end) {   // byte offset of the row of x behind row m of y (uniform)
+        if (m >= end) return kOut;
+        const int t = g.rows ? uniform_load(g.rows, m) : m;
+        return t >= 0 && t < g.T ? t * K * 2 : kOut;
+    };
+    u4_t xv[CG][XI];
+    // load i of a slice is piece lane % 32 (16 bytes) of row 2 i + lane / 32; rows that do not exist and pieces past K
+    // are zeros without a memory access
+    auto load_x = [&](const OpsItem &it, int gi) {
+        const int step = it.chunk * W + wave;
+        const bool ok = it.n > 0 && step < n_steps;
+        const int piece = (int)threadIdx.x & 31;
+        const bool inside = step * 256 + piece * 8 < K;
+#pragma unroll
+        for (int i = 0; i < XI; i++) {
+            const int m = it.row + gi * CM + 2 * i;
+            const int b0 = ok ? x_base(m, it.row_end) : kOut, b1 = ok ? x_base(m + 1, it.row_end) : kOut;
+            const int b = ((int)threadIdx.x & 32) ? b1 : b0;
+            xv[gi][i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, inside && b != kOut ? b + piece * 16 : kOut, ok ? step * 512 : 0, 0);
+        }
+    };
+    // the wave's piece, addressed as in gemv_f16d_kernel
+    const uint32_t piece = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + wave * kPiece);
+    auto xs_w = [&]() { return piece + (uint32_t)((lane >> 5) * 512 + (((lane & 31) ^ (lane >> 5)) << 4)); };
+    const int xr_row = c16 & (CM - 1);
+    const uint32_t xs_r = piece + (uint32_t)(xr_row * 512 + (((8 * q) ^ xr_row) << 4));
+
+    const int voff = c16 * row_bytes + q * 16;
+    auto issue = [&](u4_t &cwd, const OpsItem &it, int t) {
+        const int step = it.chunk * W + wave;
+        const bool ok = t < (kGated ? 2 * it.n : it.n) && step < n_steps;
+        const __amdgpu_buffer_rsrc_t crsrc = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t *>(codes) + (int64_t)it.expert * w_rows * (K >> 3), 0, w_rows * row_bytes, 0x00020000);
+        const int wrow = kGated ? (it.unit + (t >> 1)) * 16 + (t & 1) * N : (it.unit + t) * 16;
+        cwd = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? wrow * row_bytes + step * 64 : kOut, 0);
+    };
+
+    OpsItem it = next_job();
+#pragma unroll
+    for (int gi = 0; gi < CG; gi++) load_x(it, gi);
+    u4_t cw[D];
+    issue(cw[0], it, 0);   // the rest of the ring after the prologue's work, as in gemv_f16d_kernel
+    stream_stage_signs<64 * W>(smem_raw, tid);
+    __builtin_amdgcn_sched_barrier(0);
+    stream_stage_grid<64 * W>(smem_raw, grow, tid);
+#pragma unroll
+    for (int d = 1; d < D; d++) issue(cw[d], it, d);
+    __syncthreads();
+
+    f4_t acc[NT][CG];
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int gi = 0; gi < CG; gi++) acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
+
+    while (it.n > 0) {
+        const OpsItem nx = next_item(it);
+        const bool step_ok = it.chunk * W + wave < n_steps;
+        const int nt = kGated ? 2 * it.n : it.n;
+        u4_t xb[CG][8];
+#pragma unroll
+        for (int gi = 0; gi < CG; gi++) {
+#pragma unroll
+            for (int i = 0; i < XI; i++) lds_write16((xs_w() ^ (uint32_t)(32 * i)) + (uint32_t)(1024 * i), xv[gi][i]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) xb[gi][i] = lds_read16(xs_r ^ (uint32_t)(16 * i));
+            load_x(nx, gi);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (step_ok && t < nt) fd_tile_step<kAhead, CG>(cw[t % D], lane_base, quarter_bits, xb, acc[t]);
+            if (t + D < NT) issue(cw[t % D], it, t + D);
+            else issue(cw[t % D], nx, t + D - NT);
+        }
+        if (it.chunk + 1 == n_chunks) {
+            // the end of a job: cell (tile, quarter, column) of every wave's piece, a group of rows at a time
+            const const_rows_args_t *late = rows_args_late();
+            Epi epi;
+            epi.bias = late->epi.bias;
+            epi.residual = late->epi.residual;
+            epi.y = late->epi.y;
+            epi.scales = late->epi.scales;
+            epi.scale = late->epi.scale;
+            epi.scale_up = late->epi.scale_up;
+            epi.N = late->epi.N;
+            epi.act = late->epi.act;
+            epi.scale_cols = late->epi.scale_cols;
+            epi.bias_f32 = late->epi.bias_f32;
+            epi.residual_f32 = late->epi.residual_f32;
+            epi.out_f32 = late->epi.out_f32;
+            epi.vec = late->epi.vec;
+            const EpiScale sc = epi_scale(epi, it.expert);
+#pragma unroll
+            for (int gi = 0; gi < CG; gi++) {
+                if (gi > 0) __syncthreads();   // the readers of the group before are done with the pieces
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (t < nt && c16 < CM) lds_write16(piece + (uint32_t)((t * 4 + q) * CM + c16) * 16, __builtin_bit_cast(u4_t, acc[t][gi]));
+                    acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
+                }
+                __syncthreads();
+                for (int cell = tid; cell < it.n * 4 * CM; cell += 64 * W) {
+                    const int u = cell / (4 * CM), rem = cell % (4 * CM);
+                    const uint32_t src = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + ((kGated ? 2 * u : u) * 4 * CM + rem) * 16);
+                    f4_t v = __builtin_bit_cast(f4_t, lds_read16(src)), up = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+                    for (int w = 1; w < W; w++) v += __builtin_bit_cast(f4_t, lds_read16(src + w * kPiece));
+                    if constexpr (kGated) {
+                        up = __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16));
+#pragma unroll 4
+                        for (int w = 1; w < W; w++) up += __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16 + w * kPiece));
+                    }
+                    const int m = it.row + gi * CM + rem % CM;
+                    if (m < it.row_end) epi_store4<kGated, true>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
+                }
+            }
+            __syncthreads();   // the pieces take the x of the next job next
+        }
+        it = nx;
+    }
+}

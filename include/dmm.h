@@ -327,6 +327,12 @@ int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const 
                               const dmm_epilogue *epilogue, void *y, int64_t R, int64_t E, int64_t N, int64_t K,
                               void *stream);
 
+/* Forces a kernel of the two products where the library would choose, process-wide, for tests and measurement:
+ * 0 the catch-all, 1 the kernel for few rows, 2 the matrix-matrix kernel, 3 the same with split K (where a
+ * workspace is given); -1: the library's own choice.  A forced kernel that cannot take a call leaves it to one that
+ * can.  Returns the previous value (>= -1), or DMM_ERR_BAD_SHAPE.  Results differ by the order of the sums only. */
+int dmm_set_ops_kernel(int kernel);
+
 /* The choice of experts: for every row of logits [T,E] (half, bfloat16 or float) the k largest, largest first, equal ones
  * by index; a logit of -inf (or NaN) is never chosen, so a row may have fewer than k choices or none.
  *   weights  float [T,k]: softmax over the row (DMM_SCORE_SOFTMAX) or 1 / (1 + exp(-v)) (DMM_SCORE_SIGMOID) of the

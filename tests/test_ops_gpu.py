@@ -18,6 +18,15 @@ def dev(*ts):
     return [t.to(DEV) if t is not None else None for t in ts]
 
 
+@pytest.fixture(params=[-1, 1, 2, 3], ids=["auto", "rows", "gemm", "split"])
+def kernel(request):
+    """The library's choice, and every kernel in its place where it can take the call."""
+    lib = capi.lib()
+    lib.dmm_set_ops_kernel(request.param)
+    yield request.param
+    lib.dmm_set_ops_kernel(-1)
+
+
 def check_fused(M, N, K, gated=False, act="none", bias=None, residual=None, out=F16, seed=0, fp8=True, scale=None):
     x, codes, grid, b, r = fused_inputs(M, N, K, gated, bias, residual, seed + M + N + K, fp8=fp8)
     s = 1.0 / math.sqrt(max(K, 1)) if scale is None else scale
@@ -40,7 +49,7 @@ def test_fused_any_shape(M, N, K, gated):
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("bias,residual,out", [(None, None, F16), (F16, F32, F16), (F32, F16, F32), (None, F16, F16)])
-def test_fused_epilogues(act, gated, bias, residual, out):
+def test_fused_epilogues(act, gated, bias, residual, out, kernel):
     check_fused(1, 272, 512, gated, act, bias, residual, out)
     check_fused(7, 272, 512, gated, act, bias, residual, out)
     check_fused(40, 272, 512, gated, act, bias, residual, out)
@@ -48,7 +57,7 @@ def test_fused_epilogues(act, gated, bias, residual, out):
 
 @pytest.mark.parametrize("M", [1, 2, 4, 5, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 129, 300])
 @pytest.mark.parametrize("N,K,gated", [(64, 256, False), (100, 768, True), (17, 320, False), (1030, 1024, True), (515, 2112, False)])
-def test_fused_rows(M, N, K, gated):
+def test_fused_rows(M, N, K, gated, kernel):
     check_fused(M, N, K, gated, "gelu_tanh", F16, None, F16)
 
 
@@ -64,7 +73,7 @@ def test_fused_grid_that_does_not_fit_8_bits(M):
 
 
 @pytest.mark.parametrize("M", [1, 4, 16, 40])
-def test_fused_x_that_is_not_finite_stays_in_its_row(M):
+def test_fused_x_that_is_not_finite_stays_in_its_row(M, kernel):
     x, codes, grid, _, _ = fused_inputs(M, 4240, 512, False, None, None, seed=5)
     x[M - 1, 500] = math.inf
     y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.05)
@@ -137,25 +146,25 @@ COUNTS = [(1,), (0, 1), (3, 0, 0, 4, 1), (0, 0, 0), (17, 1, 0, 33, 5, 16), (1,) 
 
 @pytest.mark.parametrize("counts", COUNTS)
 @pytest.mark.parametrize("N,K,gated", [(64, 256, False), (36, 512, True), (21, 320, False), (272, 1024, True)])
-def test_grouped(counts, N, K, gated):
+def test_grouped(counts, N, K, gated, kernel):
     check_grouped(counts, 11, N, K, gated, "silu" if gated else "none", F16 if gated else None, gather=True, behind=3)
 
 
 @pytest.mark.parametrize("counts", [(3, 0, 0, 4, 1), (40, 0, 25)])
 @pytest.mark.parametrize("K", [8, 24, 264, 64, 4096])
-def test_grouped_row_order_and_types(counts, K):
+def test_grouped_row_order_and_types(counts, K, kernel):
     E = len(counts)
     check_grouped(counts, 5, 20, K, False, "gelu", F32, gather=False, behind=1, out=F32, scale=torch.linspace(0.02, 0.05, E))
     check_grouped(counts, 5, 20, K, True, "relu", F16, gather=True, out=F32, scale=torch.linspace(0.02, 0.05, 2 * E).view(E, 2))
 
 
-def test_grouped_many_tiles_per_workgroup():
+def test_grouped_many_tiles_per_workgroup(kernel):
     check_grouped((2, 0, 1, 19), 9, 8200, 256, False, "none", None)
     check_grouped((2, 0, 1, 19), 9, 4100, 512, True, "silu", None)
     check_grouped((1,), 3, 33000, 256, False, "none", None)
 
 
-def test_grouped_lists_that_lead_out_of_the_buffers():
+def test_grouped_lists_that_lead_out_of_the_buffers(kernel):
     for counts in ((2, 3), (90, 60)):
         x, codes, grid, offsets, rows, _ = grouped_inputs(counts, 4, 64, 256, False, None, True, seed=3)
         R = rows.shape[0]
