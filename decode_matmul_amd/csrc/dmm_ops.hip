@@ -89,7 +89,7 @@ int64_t dmm_route_workspace_bytes(int64_t T, int64_t E)
 {
     if (T < 1 || E < 1 || E > kRouteMaxE) return 0;
     const int64_t blocks = route_blocks(T);
-    return blocks == 1 ? 0 : blocks * E * (8 * route_words(T) + 4);
+    return blocks == 1 ? 0 : E * (blocks * 8 * route_words(T) + (blocks + 3) / 4 * 16);
 }
 
 int dmm_route_experts(const void *logits, int logits_type, int64_t T, int64_t E, int64_t k, int scoring, int normalize, void *weights,
@@ -118,13 +118,23 @@ int dmm_route_experts(const void *logits, int logits_type, int64_t T, int64_t E,
     a.rows = (int32_t *)rows;
     a.slots = (int32_t *)slots;
     a.words = T > 0 ? route_words(T) : 1;
-    a.masks = (uint64_t *)workspace;
-    a.counts = blocks > 1 ? (int32_t *)((char *)workspace + blocks * E * 8 * a.words) : nullptr;
-    if (E <= 64) return launch_route<1>(a, blocks, (hipStream_t)stream);
-    if (E <= 128) return launch_route<2>(a, blocks, (hipStream_t)stream);
-    if (E <= 256) return launch_route<4>(a, blocks, (hipStream_t)stream);
-    if (E <= 512) return launch_route<8>(a, blocks, (hipStream_t)stream);
-    return launch_route<16>(a, blocks, (hipStream_t)stream);
+    a.blocks4 = (int)((blocks + 3) / 4 * 4);
+    // the counts first: rows of a multiple of 16 bytes, so that the masks behind them are aligned too
+    a.counts = (int32_t *)workspace;
+    a.masks = blocks > 1 ? (uint64_t *)((char *)workspace + E * a.blocks4 * 4) : nullptr;
+    hipStream_t s = (hipStream_t)stream;
+    if (k <= 16 && E <= 256) {
+        if (E <= 16) return launch_route<1, 16>(a, blocks, s);
+        if (E <= 32) return launch_route<2, 16>(a, blocks, s);
+        if (E <= 64) return launch_route<4, 16>(a, blocks, s);
+        if (E <= 128) return launch_route<8, 16>(a, blocks, s);
+        return launch_route<16, 16>(a, blocks, s);
+    }
+    if (E <= 64) return launch_route<1, 64>(a, blocks, s);
+    if (E <= 128) return launch_route<2, 64>(a, blocks, s);
+    if (E <= 256) return launch_route<4, 64>(a, blocks, s);
+    if (E <= 512) return launch_route<8, 64>(a, blocks, s);
+    return launch_route<16, 64>(a, blocks, s);
 }
 
 int dmm_combine_experts(const void *y, int y_type, const void *slots, const void *weights, const void *residual, int residual_type,
@@ -135,8 +145,9 @@ int dmm_combine_experts(const void *y, int y_type, const void *slots, const void
     if ((st = ensure_ready((hipStream_t)stream))) return st;
     const CombineArgs a{y, (const int32_t *)slots, (const float *)weights, residual, out, y_type == DMM_F32, residual_type == DMM_F32,
                         out_type == DMM_F32, (int)R, (int)T, (int)k, (int)N};
-    const unsigned bx = (unsigned)((N + 255) / 256), by = (unsigned)(T < 65535 ? T : 65535);
-    return launch(combine_kernel<1>, dim3(bx, by), dim3(256), 0, (hipStream_t)stream, a);
+    const unsigned bx = (unsigned)((N + 2047) / 2048), by = (unsigned)(T < 65535 ? T : 65535);
+    if (k <= 2) return launch(combine_kernel<2>, dim3(bx, by), dim3(256), 0, (hipStream_t)stream, a);
+    return launch(combine_kernel<4>, dim3(bx, by), dim3(256), 0, (hipStream_t)stream, a);
 }
 
 int dmm_decode_matmul_fused_host(const void *x, const void *codes, const void *grid, const dmm_epilogue *ep, void *y, int64_t M,

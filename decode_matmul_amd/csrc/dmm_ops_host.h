@@ -175,9 +175,11 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_ROWS(false), DMM_K_ROWS(true),
 #undef DMM_K_ROWS
 #undef DMM_K_ROWS_X
-#define DMM_K_ROUTE(EV) kinfo(route_choose_kernel<EV, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, true>, kLdsMax, false)
-        DMM_K_ROUTE(1), DMM_K_ROUTE(2), DMM_K_ROUTE(4), DMM_K_ROUTE(8), DMM_K_ROUTE(16),
+#define DMM_K_ROUTE(EV, L) kinfo(route_choose_kernel<EV, L, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, L, true>, kLdsMax, false)
+        DMM_K_ROUTE(1, 16), DMM_K_ROUTE(2, 16), DMM_K_ROUTE(4, 16), DMM_K_ROUTE(8, 16), DMM_K_ROUTE(16, 16),
+        DMM_K_ROUTE(1, 64), DMM_K_ROUTE(2, 64), DMM_K_ROUTE(4, 64), DMM_K_ROUTE(8, 64), DMM_K_ROUTE(16, 64),
 #undef DMM_K_ROUTE
+        kinfo(route_place_kernel, kLdsMax, false),
     };
     return t;
 }
@@ -193,15 +195,18 @@ inline int route_words(int64_t T)
 }
 inline int64_t route_blocks(int64_t T) { return (T + 64 * route_words(T) - 1) / (64 * route_words(T)); }
 
-template <int EV>
+template <int EV, int L>
 int launch_route(const RouteArgs &a, int64_t blocks, hipStream_t s)
 {
     const size_t masks = (size_t)a.E * a.words * 8;
     if (blocks == 1)
-        return launch(route_choose_kernel<EV, true>, dim3(1), dim3(1024), masks + (size_t)(a.E + 1) * 4, s, a);
-    const int st = launch<true, false>(route_choose_kernel<EV, false>, dim3((unsigned)blocks), dim3(1024), masks, s, a);
+        return launch(route_choose_kernel<EV, L, true>, dim3(1), dim3(1024), masks + (size_t)(a.E + 1 + 64 * a.k) * 4, s, a);
+    const int st = launch<true, false>(route_choose_kernel<EV, L, false>, dim3((unsigned)blocks), dim3(1024), masks, s, a);
     if (st != 0) return st;
-    return launch<false, true>(route_place_kernel, dim3((unsigned)blocks), dim3(1024), (size_t)(3 * a.E + 1) * 4, s, a);
+    int parts = 0;   // lanes per expert, a power of two up to 64
+    while (parts < 6 && (2 << parts) * a.E <= 1024) parts++;
+    return launch<false, true>(route_place_kernel, dim3((unsigned)blocks), dim3(1024), masks + (size_t)(2 * a.E + 1) * 4, s, a, (int)blocks,
+                               parts);
 }
 
 // ------------------------------------------------------------------ the operators on host memory

@@ -145,7 +145,7 @@ def route64(logits, k, scoring, normalize):
         order = sorted((e for e in range(E) if v[e] > -math.inf), key=lambda e: (-v[e], e))[:k]
         if not order:
             continue
-        p = [1 / (1 + math.exp(-v[e])) for e in order] if scoring == "sigmoid" else [math.exp(v[e] - v[order[0]]) for e in order]
+        p = [1 / (1 + math.exp(-v[e])) if v[e] > 0 else math.exp(v[e]) / (1 + math.exp(v[e])) for e in order] if scoring == "sigmoid" else [math.exp(v[e] - v[order[0]]) for e in order]
         total = sum(p) if normalize else 1.0 if scoring == "sigmoid" else sum(math.exp(u - v[order[0]]) for u in v)
         for j, e in enumerate(order):
             experts[t, j] = e

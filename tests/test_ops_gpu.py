@@ -192,7 +192,8 @@ def test_grouped_empty():
 # ----------------------------------------------------------------- choice of experts
 @pytest.mark.parametrize("scoring,normalize", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
 @pytest.mark.parametrize("T,E,k,dtype", [(1, 1, 1, F32), (5, 8, 2, F16), (64, 64, 6, F32), (65, 65, 7, torch.bfloat16), (3, 12, 12, F32),
-                                         (200, 128, 8, F16), (300, 257, 5, F32), (70, 1000, 64, F16), (130, 600, 3, F32)])
+                                         (200, 128, 8, F16), (300, 257, 5, F32), (70, 1000, 64, F16), (130, 600, 3, F32),
+                                         (90, 16, 16, F16), (67, 30, 17, F32), (61, 200, 16, F32), (63, 100, 40, F16), (66, 40, 4, F16)])
 def test_route(T, E, k, dtype, scoring, normalize):
     gen = torch.Generator().manual_seed(T + E)
     logits = (torch.randn(T, E, generator=gen) * 2).to(dtype)
