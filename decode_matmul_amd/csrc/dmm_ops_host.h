@@ -84,13 +84,13 @@ int run_ops_gemm(const void *x, const void *codes, const void *grid, const Group
 std::atomic<int> g_ops_kernel{-1};
 enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3 };
 
-template <int NT, int XI, int W, int CG, bool kGated>
+template <int NT, int XI, int W, int CG, bool kGated, bool kOne>
 int launch_ops_rows_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
                          hipStream_t s)
 {
     const int64_t wgs = units < cu_count() ? units : cu_count();
-    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K};
-    return launch(ops_rows_kernel<NT, 2, XI, W, CG, kGated>, dim3((unsigned)wgs), dim3(64 * W), (size_t)fd_lds_bytes(XI, W), s, args);
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, (int)(units / wgs), (int)(units % wgs)};
+    return launch(ops_rows_kernel<NT, 2, XI, W, CG, kGated, kOne>, dim3((unsigned)wgs), dim3(64 * W), (size_t)fd_lds_bytes(XI, W), s, args);
 }
 
 // most segments the rows can make, sr rows each: an expert adds at most one cut one, and none without a row
@@ -105,9 +105,14 @@ int launch_ops_rows(const void *x, const void *codes, const void *grid, const Gr
 {
     const int64_t units = ops_segments(g, 2 * XI * CG) * ((e.N + 15) / 16);
     const int64_t cus = cu_count(), share = (units + cus - 1) / cus * (kGated ? 2 : 1);   // most tiles a workgroup gets
-    if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
-    if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
-    return launch_ops_rows_inst<8, XI, W, CG, kGated>(x, codes, grid, g, e, K, units, s);
+    if (!g.offsets && g.R <= 2 * XI * CG && share <= 8) {
+        if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated, true>(x, codes, grid, g, e, K, units, s);
+        if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated, true>(x, codes, grid, g, e, K, units, s);
+        return launch_ops_rows_inst<8, XI, W, CG, kGated, true>(x, codes, grid, g, e, K, units, s);
+    }
+    if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
+    if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
+    return launch_ops_rows_inst<8, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
 }
 
 // rows of a segment by the rows an expert has
@@ -168,11 +173,11 @@ const std::vector<KernelInfo> &ops_kernel_table()
         kinfo(ops_gemm_kernel<4, G>, gr_smem_bytes(4), true)
         DMM_K_OPS(false), DMM_K_OPS(true),
 #undef DMM_K_OPS
-#define DMM_K_ROWS_X(NT, G)                                                                                             \
-    kinfo(ops_rows_kernel<NT, 2, 2, 16, 1, G>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 4, 16, 1, G>, kLdsMax, true), \
-        kinfo(ops_rows_kernel<NT, 2, 8, 8, 1, G>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 8, 8, 2, G>, kLdsMax, true)
-#define DMM_K_ROWS(G) DMM_K_ROWS_X(2, G), DMM_K_ROWS_X(4, G), DMM_K_ROWS_X(8, G)
-        DMM_K_ROWS(false), DMM_K_ROWS(true),
+#define DMM_K_ROWS_X(NT, G, O)                                                                                                    \
+    kinfo(ops_rows_kernel<NT, 2, 2, 16, 1, G, O>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 4, 16, 1, G, O>, kLdsMax, true),   \
+        kinfo(ops_rows_kernel<NT, 2, 8, 8, 1, G, O>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 8, 8, 2, G, O>, kLdsMax, true)
+#define DMM_K_ROWS(G, O) DMM_K_ROWS_X(2, G, O), DMM_K_ROWS_X(4, G, O), DMM_K_ROWS_X(8, G, O)
+        DMM_K_ROWS(false, false), DMM_K_ROWS(true, false), DMM_K_ROWS(false, true), DMM_K_ROWS(true, true),
 #undef DMM_K_ROWS
 #undef DMM_K_ROWS_X
 #define DMM_K_ROUTE(EV, L) kinfo(route_choose_kernel<EV, L, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, L, true>, kLdsMax, false)

@@ -26,8 +26,9 @@ typedef __attribute__((address_space(4))) const int32_t const_i32_t;
 // an element of a list that no kernel writes meanwhile, at the same place in all lanes: through the scalar cache
 __device__ __forceinline__ int uniform_load(const int32_t *p, int i)
 {
-    return reinterpret_cast<const_i32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+    return __builtin_amdgcn_readfirstlane(reinterpret_cast<const_i32_t *>(reinterpret_cast<uintptr_t>(p))[i]);
 }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ GroupRange uniform_range(const Groups &g, int e)
 {
@@ -127,6 +128,7 @@ struct OpsRowsArgs {
     Groups g;
     Epi epi;
     int K;
+    int units_q, units_r;   // dense calls of one segment: units per workgroup, one more for the first units_r
 };
 typedef __attribute__((address_space(4))) const OpsRowsArgs const_rows_args_t;
 
@@ -138,7 +140,10 @@ __device__ __forceinline__ const_rows_args_t *rows_args_late()
 }
 
 // XI, W, CG as in gemv_f16d_kernel: 2 XI rows of x per group, W waves, CG groups of sixteen rows per segment.
-template <int NT, int D, int XI, int W, int CG, bool kGated>
+// kOne: a dense call of one segment whose workgroups have one job each (up to NU units): the range comes from the
+// host, rows of x follow each other, and the loop has only chunks to count.  As a job of the general form 4096 x 11008
+// with one row took 8.1 us, like this 6.x.
+template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne>
 __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
 {
     const uint16_t *__restrict__ x = args.x;
@@ -172,8 +177,16 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
     constexpr int kOut = (int)0x80000000;
 
     const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
-    OpsCursor cur;
-    if (!ops_range<SR, NU>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
+    OpsCursor cur{};
+    if constexpr (kOne) {
+        const int b = (int)blockIdx.x;
+        cur.unit = b * args.units_q + (b < args.units_r ? b : args.units_r);
+        cur.left = args.units_q + (b < args.units_r ? 1 : 0);
+        cur.row_end = g.R;
+    } else {
+        if (!ops_range<SR, NU>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
+        cur = OpsCursor{uniform(cur.expert), uniform(cur.row), uniform(cur.row_end), uniform(cur.unit), uniform(cur.left), uniform(cur.per)};
+    }
 
     // the next job, and the cursor behind it
     auto next_job = [&]() {
@@ -199,6 +212,10 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
     };
     auto next_item = [&](const OpsItem &it) {
         OpsItem o = it;
+        if constexpr (kOne) {
+            o.chunk++;
+            return o;
+        }
         if (it.n > 0 && it.chunk + 1 < n_chunks) o.chunk++;
         else o = next_job();
         return o;
@@ -219,6 +236,13 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
         const bool ok = it.n > 0 && step < n_steps;
         const int piece = (int)threadIdx.x & 31;
         const bool inside = step * 256 + piece * 8 < K;
+        if constexpr (kOne) {   // rows past the last lie past the end of the buffer
+            const int b = inside ? ((((int)threadIdx.x >> 5) & 1) * K + piece * 8) * 2 : kOut;
+#pragma unroll
+            for (int i = 0; i < XI; i++)
+                xv[gi][i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, b, ok ? step * 512 + (gi * CM + 2 * i) * 2 * K : kOut, 0);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < XI; i++) {
             const int m = it.row + gi * CM + 2 * i;
@@ -243,7 +267,9 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
         cwd = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? wrow * row_bytes + step * 64 : kOut, 0);
     };
 
-    OpsItem it = next_job();
+    OpsItem it;
+    if constexpr (kOne) it = OpsItem{0, 0, g.R, cur.unit, cur.left, 0};
+    else it = next_job();
 #pragma unroll
     for (int gi = 0; gi < CG; gi++) load_x(it, gi);
     u4_t cw[D];
@@ -261,7 +287,9 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
 #pragma unroll
         for (int gi = 0; gi < CG; gi++) acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
 
-    while (it.n > 0) {
+    while (kOne ? it.chunk < n_chunks : it.n > 0) {
+        // (a value of its own every time round: what depends on it is not kept in scalar registers through the loop)
+        asm volatile("" : "+s"(it.n), "+s"(it.unit));
         const OpsItem nx = next_item(it);
         const bool step_ok = it.chunk * W + wave < n_steps;
         const int nt = kGated ? 2 * it.n : it.n;
@@ -322,7 +350,7 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
                     if (m < it.row_end) epi_store4<kGated, true>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
                 }
             }
-            __syncthreads();   // the pieces take the x of the next job next
+            if constexpr (!kOne) __syncthreads();   // the pieces take the x of the next job next
         }
         it = nx;
     }
