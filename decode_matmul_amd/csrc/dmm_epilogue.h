@@ -119,16 +119,17 @@ __device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, con
     if (n >= e.N) return;
     const int left = e.N - n;   // outputs that exist, from here on
     const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
-    f4_t z = v * sc.s;
-    if (e.bias) z += epi_load4(e.bias, b, e.bias_f32, e.vec, left);
-    z = epi_act4<kSmall>(z, e.act);
-    if (kGated) {
-        f4_t w = u * sc.up;
-        if (e.bias) w += epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
-        z *= w;
-    }
     const int64_t i = row * e.N + n;
-    if (e.residual) z += epi_load4(e.residual, i, e.residual_f32, e.vec, left);
+    // every operand is asked for before the first is used
+    f4_t bz = f4_t{0.f, 0.f, 0.f, 0.f}, bu = bz, rs = bz;
+    if (e.bias) {
+        bz = epi_load4(e.bias, b, e.bias_f32, e.vec, left);
+        if (kGated) bu = epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
+    }
+    if (e.residual) rs = epi_load4(e.residual, i, e.residual_f32, e.vec, left);
+    f4_t z = epi_act4<kSmall>(v * sc.s + bz, e.act);
+    if (kGated) z *= u * sc.up + bu;
+    if (e.residual) z += rs;
     if (!e.vec) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {

@@ -154,6 +154,7 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
     constexpr int SR = CG * CM;          // rows of a segment
     constexpr int kPiece = XI * 1024;
     constexpr int NU = kGated ? NT / 2 : NT;
+    constexpr int kSumUnroll = kOne ? 8 : 4;   // a job with others behind it has their loads in registers: fewer sums side by side
     static_assert((W == 16 && (XI == 2 || XI == 4)) || (W == 8 && XI == 8), "up to four, eight or sixteen rows of x");
     static_assert(CG == 1 || (CG == 2 && XI == 8), "a second group of rows only beside a full first one");
     static_assert(fd_lds_bytes(XI, W) <= 160 * 1024, "tables and pieces have to fit the LDS");
@@ -337,17 +338,17 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
                 __syncthreads();
                 for (int cell = tid; cell < it.n * 4 * CM; cell += 64 * W) {
                     const int u = cell / (4 * CM), rem = cell % (4 * CM);
-                    const uint32_t src = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + ((kGated ? 2 * u : u) * 4 * CM + rem) * 16);
-                    f4_t v = __builtin_bit_cast(f4_t, lds_read16(src)), up = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-                    for (int w = 1; w < W; w++) v += __builtin_bit_cast(f4_t, lds_read16(src + w * kPiece));
-                    if constexpr (kGated) {
-                        up = __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16));
-#pragma unroll 4
-                        for (int w = 1; w < W; w++) up += __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16 + w * kPiece));
-                    }
                     const int m = it.row + gi * CM + rem % CM;
-                    if (m < it.row_end) epi_store4<kGated, true>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
+                    if (m >= it.row_end) continue;
+                    const uint32_t src = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + ((kGated ? 2 * u : u) * 4 * CM + rem) * 16);
+                    f4_t v = f4_t{0.f, 0.f, 0.f, 0.f}, up = v;
+#pragma unroll kSumUnroll
+                    for (int w = 0; w < W; w++) v += __builtin_bit_cast(f4_t, lds_read16(src + w * kPiece));
+                    if constexpr (kGated) {
+#pragma unroll kSumUnroll
+                        for (int w = 0; w < W; w++) up += __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16 + w * kPiece));
+                    }
+                    epi_store4<kGated, (W == 16)>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
                 }
             }
             if constexpr (!kOne) __syncthreads();   // the pieces take the x of the next job next
