@@ -374,7 +374,7 @@ std::atomic<int> g_choice[4] = {{-1}, {-1}, {-1}, {-1}};
 // environment (read once, at the first call that needs it) for hosts that cannot call it.
 std::atomic<int> g_gemv_q8{-1};
 
-inline bool gemv_q8_enabled()
+bool gemv_q8_enabled()
 {
     int on = g_gemv_q8.load(std::memory_order_relaxed);
     if (on < 0) {

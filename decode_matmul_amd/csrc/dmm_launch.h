@@ -56,3 +56,5 @@ bool gemm_reg_ok(int64_t M, int64_t N, int64_t K);
 int splitk_plan(int64_t M, int64_t N, int64_t K, int64_t workspace_bytes, int cus);
 int launch_gemm_partial(const void *x, const void *codes, const void *grid, float *part, int splits, int64_t M, int64_t N, int64_t K,
                         hipStream_t stream);
+
+bool gemv_q8_enabled();   // dmm_set_gemv_8bit: may the library pick kernels on 8-bit operands?

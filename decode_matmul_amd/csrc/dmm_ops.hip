@@ -25,6 +25,8 @@ namespace dmm {
 #include "dmm_hostroute.h"
 #include "dmm_tables.h"
 #include "dmm_gemv_f16.h"
+#include "dmm_gemv_q8.h"
+#include "dmm_gemv_q8d.h"
 #include "dmm_gemv_f16d.h"
 #include "dmm_gemm.h"
 #include "dmm_epilogue.h"
@@ -54,7 +56,7 @@ int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, 
 
 int dmm_set_ops_kernel(int kernel)
 {
-    if (kernel < -1 || kernel > kOpsSplit) return DMM_ERR_BAD_SHAPE;
+    if (kernel < -1 || kernel > kOpsRows8) return DMM_ERR_BAD_SHAPE;
     return g_ops_kernel.exchange(kernel, std::memory_order_relaxed);
 }
 

@@ -82,7 +82,7 @@ int run_ops_gemm(const void *x, const void *codes, const void *grid, const Group
 
 // dmm_set_ops_kernel: what a test or a benchmark forces instead of the choice below (-1: nothing)
 std::atomic<int> g_ops_kernel{-1};
-enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3 };
+enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3, kOpsRows8 = 4 };
 
 template <int NT, int XI, int W, int CG, bool kGated, bool kOne>
 int launch_ops_rows_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
@@ -115,6 +115,30 @@ int launch_ops_rows(const void *x, const void *codes, const void *grid, const Gr
     return launch_ops_rows_inst<8, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
 }
 
+template <int NT, bool kGated, bool kOne>
+int launch_ops_rows8_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
+                          hipStream_t s)
+{
+    const int64_t wgs = units < cu_count() ? units : cu_count();
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, (int)(units / wgs), (int)(units % wgs)};
+    return launch(ops_rows8_kernel<NT, 2, kGated, kOne>, dim3((unsigned)wgs), dim3(1024), (size_t)kO8Bytes, s, args);
+}
+
+// 8-bit operands, two rows per segment
+template <bool kGated>
+int run_ops_rows8(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t units = ops_segments(g, 2) * ((e.N + 15) / 16);
+    const int64_t cus = cu_count(), share = (units + cus - 1) / cus * (kGated ? 2 : 1);
+    if (!g.offsets && g.R <= 2 && share <= 8) {
+        if (share <= 2) return launch_ops_rows8_inst<2, kGated, true>(x, codes, grid, g, e, K, units, s);
+        if (share <= 4) return launch_ops_rows8_inst<4, kGated, true>(x, codes, grid, g, e, K, units, s);
+        return launch_ops_rows8_inst<8, kGated, true>(x, codes, grid, g, e, K, units, s);
+    }
+    if (share <= 4) return launch_ops_rows8_inst<4, kGated, false>(x, codes, grid, g, e, K, units, s);
+    return launch_ops_rows8_inst<8, kGated, false>(x, codes, grid, g, e, K, units, s);
+}
+
 // rows of a segment by the rows an expert has
 template <bool kGated>
 int run_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
@@ -133,7 +157,9 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
     if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
-    const bool rows_ok = ops_segments(g, 4) * ((e.N + 15) / 16) < (1LL << 31);
+    const bool rows_ok = ops_segments(g, 2) * ((e.N + 15) / 16) < (1LL << 31);
+    if (rows_ok && !e.out_f32 && (force == kOpsRows8 || (force < 0 && g.R <= 2 && gemv_q8_enabled())))
+        return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && (force == kOpsRows || (force < 0 && g.R / g.E <= 32))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
     if (force != kOpsGemm && !g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 &&
         gemm_reg_ok(g.R, rows, K)) {
@@ -180,6 +206,12 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_ROWS(false, false), DMM_K_ROWS(true, false), DMM_K_ROWS(false, true), DMM_K_ROWS(true, true),
 #undef DMM_K_ROWS
 #undef DMM_K_ROWS_X
+#define DMM_K_ROWS8(G)                                                                                                            \
+    kinfo(ops_rows8_kernel<2, 2, G, true>, kLdsMax, true), kinfo(ops_rows8_kernel<4, 2, G, true>, kLdsMax, true),                 \
+        kinfo(ops_rows8_kernel<8, 2, G, true>, kLdsMax, true), kinfo(ops_rows8_kernel<4, 2, G, false>, kLdsMax, true),            \
+        kinfo(ops_rows8_kernel<8, 2, G, false>, kLdsMax, true)
+        DMM_K_ROWS8(false), DMM_K_ROWS8(true),
+#undef DMM_K_ROWS8
 #define DMM_K_ROUTE(EV, L) kinfo(route_choose_kernel<EV, L, false>, kLdsMax, false), kinfo(route_choose_kernel<EV, L, true>, kLdsMax, false)
         DMM_K_ROUTE(1, 16), DMM_K_ROUTE(2, 16), DMM_K_ROUTE(4, 16), DMM_K_ROUTE(8, 16), DMM_K_ROUTE(16, 16),
         DMM_K_ROUTE(1, 64), DMM_K_ROUTE(2, 64), DMM_K_ROUTE(4, 64), DMM_K_ROUTE(8, 64), DMM_K_ROUTE(16, 64),

@@ -139,25 +139,79 @@ __device__ __forceinline__ const_rows_args_t *rows_args_late()
     return reinterpret_cast<const_rows_args_t *>((uintptr_t)p);
 }
 
-// XI, W, CG as in gemv_f16d_kernel: 2 XI rows of x per group, W waves, CG groups of sixteen rows per segment.
+// ---- 8-bit operands (gemv_q8d_kernel's arithmetic) for segments of up to two rows.  The sixteen columns of the
+// matrix unit hold four terms of each row (column 4 m + t is term t of row m, of weight 8^-t), the means of the shift
+// term ride in columns 4 m and 4 m + 1.  A wave splits the 256 k of its own step into terms - a lane has one piece
+// of eight, lanes 32 .. 63 those of the second row - and leaves them in its own piece of LDS: term row 4 m + t at a
+// pitch of 272 bytes, the means behind them at a pitch of 80; no barrier, no roles.  What does not fit is found, not
+// computed: a grid fp8 cannot hold sends the workgroup to the 16-bit body before it starts, a row of x that is
+// not finite sends the job, at its end, through rows_job_slow.
+constexpr int kO8TermPitch = 272, kO8MeanPitch = 80;
+constexpr int kO8Means = 8 * kO8TermPitch;
+constexpr int kO8Piece = kO8Means + 4 * kO8MeanPitch + 64;   // 2560
+constexpr int kO8Flags = kSTablesBytes + 16 * kO8Piece;      // 16 votes, 2 words for jobs that are not finite, 64 zero bytes
+constexpr int kO8Bytes = kO8Flags + 128 + 64;
+static_assert(kO8Bytes <= 160 * 1024, "tables and pieces have to fit the LDS");
+
+// A job's outputs one by one, weights decoded from the grid in memory, dot products on the vector ALU: what a job whose
+// x is not finite gets (the terms of an infinity mean nothing).  Any x, the 16-bit kernels' arithmetic.
+template <bool kGated, int W>
+__device__ __forceinline__ void rows_job_slow(const OpsRowsArgs &a, const Epi &epi, int expert, int row, int row_end, int unit, int n, int wave,
+                                           int lane)
+{
+    constexpr int kH = kGated ? 2 : 1;
+    const int kc = a.K >> 3;
+    const uint16_t *ce = a.codes + (int64_t)expert * kH * epi.N * kc;
+    const EpiScale sc = epi_scale(epi, expert);
+    for (int i = wave; i < n * 16; i += W) {
+        const int col = unit * 16 + i;
+        if (col >= epi.N) break;
+        for (int m = row; m < row_end; m++) {
+            const int t = group_row(a.g, m);
+            float acc[kH] = {};
+            for (int j = lane; j < kc; j += kWave) {
+                const uint16_t *xp = a.x + (int64_t)(t < 0 ? 0 : t) * a.K + j * 8;
+#pragma unroll
+                for (int h = 0; h < kH; h++) {
+                    const uint32_t c = ce[((int64_t)col + (int64_t)h * epi.N) * kc + j];
+                    const u4_t gr = reinterpret_cast<const u4_t *>(a.grid)[c & 0xFFu], sr = sign_row((c >> 8) & 0x7Fu);
+                    const h2_t d = as_h2(((c & 0x8000u) * 0x10001u) | 0x34003400u);
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const h2_t w = __builtin_elementwise_fma(as_h2(gr[p]), as_h2(sr[p]), d);
+                        const float x0 = t < 0 ? 0.f : (float)__builtin_bit_cast(half_t, xp[2 * p]);
+                        const float x1 = t < 0 ? 0.f : (float)__builtin_bit_cast(half_t, xp[2 * p + 1]);
+                        acc[h] = __builtin_fmaf(x1, (float)w[1], __builtin_fmaf(x0, (float)w[0], acc[h]));
+                    }
+                }
+            }
+            const float v = wave_sum(acc[0]), u = kGated ? wave_sum(acc[kH - 1]) : 0.f;
+            if (lane == 0) epi_store1<kGated>(epi, sc, v, u, m, col, expert);
+        }
+    }
+}
+
+// XI, W, CG as in gemv_f16d_kernel: 2 XI rows of x per group, W waves, CG groups of sixteen rows per segment; SR: rows of
+// a segment, CG * 2 XI or fewer.
 // kOne: a dense call of one segment whose workgroups have one job each (up to NU units): the range comes from the
-// host, rows of x follow each other, and the loop has only chunks to count.  As a job of the general form 4096 x 11008
-// with one row took 8.1 us, like this 6.x.
-template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne>
-__global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
+// host, rows of x follow each other, and the loop has only chunks to count (11008 -> 4096 with one row: 8.1 us as a
+// job of the general form, 6.8 like this).
+// kQ8: 8-bit operands, XI = 1; false if the grid does not fit them and nothing was done.
+template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne, int SR, bool kQ8>
+__device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
 {
     const uint16_t *__restrict__ x = args.x;
     const uint16_t *__restrict__ codes = args.codes;
     const Groups g = args.g;
     const int K = args.K, N = args.epi.N;
     constexpr int CM = 2 * XI;
-    constexpr int SR = CG * CM;          // rows of a segment
-    constexpr int kPiece = XI * 1024;
+    constexpr int kPiece = kQ8 ? kO8Piece : XI * 1024;
     constexpr int NU = kGated ? NT / 2 : NT;
     constexpr int kSumUnroll = kOne ? 8 : 4;   // a job with others behind it has their loads in registers: fewer sums side by side
-    static_assert((W == 16 && (XI == 2 || XI == 4)) || (W == 8 && XI == 8), "up to four, eight or sixteen rows of x");
+    static_assert(kQ8 ? W == 16 && XI == 1 && CG == 1 : (W == 16 && (XI == 2 || XI == 4)) || (W == 8 && XI == 8), "up to two, four, eight or sixteen rows of x");
     static_assert(CG == 1 || (CG == 2 && XI == 8), "a second group of rows only beside a full first one");
-    static_assert(fd_lds_bytes(XI, W) <= 160 * 1024, "tables and pieces have to fit the LDS");
+    static_assert(SR <= CG * CM, "the rows of a segment are columns of the product");
+    static_assert(kQ8 || fd_lds_bytes(XI, W) <= 160 * 1024, "tables and pieces have to fit the LDS");
     static_assert(NT % D == 0 && (!kGated || NT % 2 == 0), "the ring has to divide the tiles");
     static_assert(NT * 4 * CM * 16 <= kPiece, "the partial sums of a job go through the wave's piece");
     constexpr bool kAhead = W == 8 ? !(NT == 8 && CG == 2) : NT < (XI == 4 && kGated ? 4 : 8);   // a code word's gathers ahead of the word before it, where registers are left
@@ -173,7 +227,7 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
     const int row_bytes = K >> 2;
     const int w_rows = kGated ? 2 * N : N;
     const int upn = (N + 15) >> 4;
-    const uint32_t lane_base = (uint32_t)c16 * 16u;
+    const uint32_t lane_base = kQ8 ? (uint32_t)(lane & 31) * 8u : (uint32_t)c16 * 16u;
     const uint32_t quarter_bits = 0x34003400u;
     constexpr int kOut = (int)0x80000000;
 
@@ -185,7 +239,7 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
         cur.left = args.units_q + (b < args.units_r ? 1 : 0);
         cur.row_end = g.R;
     } else {
-        if (!ops_range<SR, NU>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
+        if (!ops_range<SR, NU>(g, upn, lane, cur)) return true;   // the whole workgroup, before any barrier
         cur = OpsCursor{uniform(cur.expert), uniform(cur.row), uniform(cur.row_end), uniform(cur.unit), uniform(cur.left), uniform(cur.per)};
     }
 
@@ -275,12 +329,47 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
     for (int gi = 0; gi < CG; gi++) load_x(it, gi);
     u4_t cw[D];
     issue(cw[0], it, 0);   // the rest of the ring after the prologue's work, as in gemv_f16d_kernel
-    stream_stage_signs<64 * W>(smem_raw, tid);
-    __builtin_amdgcn_sched_barrier(0);
-    stream_stage_grid<64 * W>(smem_raw, grow, tid);
+    uint32_t *flags = reinterpret_cast<uint32_t *>(smem_raw + kO8Flags);   // kQ8 only
+    if constexpr (kQ8) {
+        bool exact = true;
+        if (tid < 256) {
+            const u2_t g8 = grid_row_fp8(grow, exact);
+            const uint32_t gg = lds_addr(smem_raw) + (uint32_t)(kSSignBytes + (tid * 16 + (tid & 15)) * 16);   // slot i ^ (tid % 16)
+#pragma unroll
+            for (int i = 0; i < 16; i++) lds_write16(gg ^ (uint32_t)(i * 16), u4_t{g8[0], g8[1], g8[0], g8[1]});
+        } else if (tid < 512) {
+            const int t = tid - 256, row = t >> 1;
+            const u2_t sb = sign_bytes((uint32_t)row);
+            const uint32_t sg = lds_addr(smem_raw) + (uint32_t)((row * 16 + (t & 1) * 8 + (row & 7)) * 16);
+#pragma unroll
+            for (int i = 0; i < 8; i++) lds_write16(sg ^ (uint32_t)(i * 16), u4_t{sb[0], sb[1], sb[0], sb[1]});
+        } else if (tid < 528) {
+            flags[16 + tid - 512] = 0u;   // the two words, and what lies up to the zeros
+        } else if (tid < 544) {
+            flags[32 + tid - 528] = 0u;   // the zero bytes the idle columns read
+        }
+        const bool bad = __builtin_amdgcn_ballot_w64(!exact) != 0;
+        if (lane == 0) flags[wave] = bad ? 1u : 0u;
+    } else {
+        stream_stage_signs<64 * W>(smem_raw, tid);
+        __builtin_amdgcn_sched_barrier(0);
+        stream_stage_grid<64 * W>(smem_raw, grow, tid);
+    }
 #pragma unroll
     for (int d = 1; d < D; d++) issue(cw[d], it, d);
     __syncthreads();
+    if constexpr (kQ8) {
+        if (__builtin_amdgcn_ballot_w64(flags[lane & 15] != 0) != 0) {
+            __syncthreads();   // everybody has read the votes: the other body may have the LDS
+            return false;
+        }
+    }
+    // kQ8: this lane's column of the two B operands and of the means inside the piece; idle columns read the zeros
+    const uint32_t zeros = lds_addr(smem_raw) + (uint32_t)(kO8Flags + 128);
+    const uint32_t o8_t = c16 < 8 ? piece + (uint32_t)(c16 * kO8TermPitch + q * 64) : zeros;
+    const uint32_t o8_m = c16 < 8 && (c16 & 3) < 2 ? piece + (uint32_t)(kO8Means + ((c16 >> 2) * 2 + (c16 & 1)) * kO8MeanPitch + q * 16) : zeros;
+    bool finite = true;   // kQ8: the x of this wave's steps of the job, so far
+    int parity = 0;       // of the job
 
     f4_t acc[NT][CG];
 #pragma unroll
@@ -294,18 +383,41 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
         const OpsItem nx = next_item(it);
         const bool step_ok = it.chunk * W + wave < n_steps;
         const int nt = kGated ? 2 * it.n : it.n;
-        u4_t xb[CG][8];
+        u4_t xb[CG][kQ8 ? 1 : 8];
+        i8_t xb0{}, xb1{};
+        h8_t xm{};
+        if constexpr (kQ8) {
+            u2_t tm[4];
+            uint32_t mean;
+            finite = finite & qd_split_piece(xv[0][0], tm, mean);
+            const uint32_t m = (uint32_t)lane >> 5, pc = (uint32_t)lane & 31;
+            typedef __attribute__((address_space(3))) u2_t lds_u2_rw_t;
+            typedef __attribute__((address_space(3))) uint16_t lds_u16_rw_t;
 #pragma unroll
-        for (int gi = 0; gi < CG; gi++) {
+            for (int t = 0; t < 4; t++) *reinterpret_cast<lds_u2_rw_t *>(piece + (m * 4 + t) * kO8TermPitch + pc * 8) = tm[t];
+            *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + m * 2 * kO8MeanPitch + pc * 2) = (uint16_t)mean;
+            *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + (m * 2 + 1) * kO8MeanPitch + pc * 2) = (uint16_t)(mean >> 16);
+            const u4_t r0 = lds_read16(o8_t), r1 = lds_read16(o8_t + 16), r2 = lds_read16(o8_t + 32), r3 = lds_read16(o8_t + 48);
+            xm = __builtin_bit_cast(h8_t, lds_read16(o8_m));
+            xb0 = i8_t{(int)r0[0], (int)r0[1], (int)r0[2], (int)r0[3], (int)r1[0], (int)r1[1], (int)r1[2], (int)r1[3]};
+            xb1 = i8_t{(int)r2[0], (int)r2[1], (int)r2[2], (int)r2[3], (int)r3[0], (int)r3[1], (int)r3[2], (int)r3[3]};
+            load_x(nx, 0);
+        } else {
 #pragma unroll
-            for (int i = 0; i < XI; i++) lds_write16((xs_w() ^ (uint32_t)(32 * i)) + (uint32_t)(1024 * i), xv[gi][i]);
+            for (int gi = 0; gi < CG; gi++) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) xb[gi][i] = lds_read16(xs_r ^ (uint32_t)(16 * i));
-            load_x(nx, gi);
+                for (int i = 0; i < XI; i++) lds_write16((xs_w() ^ (uint32_t)(32 * i)) + (uint32_t)(1024 * i), xv[gi][i]);
+#pragma unroll
+                for (int i = 0; i < 8; i++) xb[gi][i] = lds_read16(xs_r ^ (uint32_t)(16 * i));
+                load_x(nx, gi);
+            }
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            if (step_ok && t < nt) fd_tile_step<kAhead, CG>(cw[t % D], lane_base, quarter_bits, xb, acc[t]);
+            if (step_ok && t < nt) {
+                if constexpr (kQ8) qd_tile_step(cw[t % D], lane_base, xb0, xb1, xm, acc[t][0]);
+                else fd_tile_step<kAhead, CG>(cw[t % D], lane_base, quarter_bits, xb, acc[t]);
+            }
             if (t + D < NT) issue(cw[t % D], it, t + D);
             else issue(cw[t % D], nx, t + D - NT);
         }
@@ -332,10 +444,37 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
                 if (gi > 0) __syncthreads();   // the readers of the group before are done with the pieces
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    if (t < nt && c16 < CM) lds_write16(piece + (uint32_t)((t * 4 + q) * CM + c16) * 16, __builtin_bit_cast(u4_t, acc[t][gi]));
+                    if (t < nt) {
+                        f4_t v = acc[t][gi];
+                        int col = c16;
+                        if constexpr (kQ8) {   // the four terms of a row, with their weights 8^-t, into the lane of column 4 m
+                            const float wt = __builtin_bit_cast(float, 0x3F800000u - (((uint32_t)c16 & 3u) * 3u << 23));
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                v[e] *= wt;
+                                v[e] = dpp_shl_add<1>(v[e], v[e]);
+                                v[e] = dpp_shl_add<2>(v[e], v[e]);
+                            }
+                            col = (c16 & 3) == 0 ? c16 >> 2 : CM;
+                        }
+                        if (col < CM) lds_write16(piece + (uint32_t)((t * 4 + q) * CM + col) * 16, __builtin_bit_cast(u4_t, v));
+                    }
                     acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
                 }
+                if constexpr (kQ8) {
+                    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && lane == 0) flags[16 + parity] = 1u;
+                    finite = true;
+                }
                 __syncthreads();
+                if constexpr (kQ8) {
+                    const bool slow = __builtin_amdgcn_ballot_w64(flags[16 + parity] != 0) != 0;
+                    parity ^= 1;
+                    if (tid == 0) flags[16 + parity] = 0u;   // read by all before this job's barrier, set again behind the next one
+                    if (slow) {
+                        rows_job_slow<kGated, W>(args, epi, it.expert, it.row, it.row_end, it.unit, it.n, wave, lane);
+                        break;
+                    }
+                }
                 for (int cell = tid; cell < it.n * 4 * CM; cell += 64 * W) {
                     const int u = cell / (4 * CM), rem = cell % (4 * CM);
                     const int m = it.row + gi * CM + rem % CM;
@@ -355,4 +494,17 @@ __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
         }
         it = nx;
     }
+    return true;
+}
+
+template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne>
+__global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
+{
+    ops_rows_body<NT, D, XI, W, CG, kGated, kOne, 2 * XI * CG, false>(args);
+}
+
+template <int NT, int D, bool kGated, bool kOne>
+__global__ __launch_bounds__(1024) void ops_rows8_kernel(OpsRowsArgs args)
+{
+    if (!ops_rows_body<NT, D, 1, 16, 1, kGated, kOne, 2, true>(args)) ops_rows_body<NT, D, 2, 16, 1, kGated, kOne, 2, false>(args);
 }

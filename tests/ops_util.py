@@ -92,17 +92,26 @@ def weights(gen, *shape, fp8=True):
     return codes, grid
 
 
-def fused_inputs(M, N, K, gated, bias, residual, seed, fp8=True):
+def rows_of_x(gen, rows, K, coarse):
+    """Normal values, or (coarse) values of two significant bits: one 8-bit term each, every product and every sum of
+    them exact on 8-bit operands too, so that the error bound of exact products holds there."""
+    if not coarse:
+        return torch.randn(rows, K, generator=gen).half()
+    pick = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, -0.5, -1.0, -1.5, -2.0, -3.0])
+    return pick[torch.randint(0, len(pick), (rows, K), generator=gen)].half()
+
+
+def fused_inputs(M, N, K, gated, bias, residual, seed, fp8=True, coarse=False):
     gen = torch.Generator().manual_seed(seed)
     n2 = 2 * N if gated else N
     codes, grid = weights(gen, n2, K // 8, fp8=fp8)
-    x = torch.randn(M, K, generator=gen).half()
+    x = rows_of_x(gen, M, K, coarse)
     b = torch.randn(n2, generator=gen).to(bias) if bias else None
     r = torch.randn(M, N, generator=gen).to(residual) if residual else None
     return x, codes, grid, b, r
 
 
-def grouped_inputs(counts, T, N, K, gated, bias, gather, seed, behind=0):
+def grouped_inputs(counts, T, N, K, gated, bias, gather, seed, behind=0, coarse=False):
     """Rows of every expert from counts, `behind` rows that belong to none."""
     gen = torch.Generator().manual_seed(seed)
     E, n2 = len(counts), 2 * N if gated else N
@@ -110,7 +119,7 @@ def grouped_inputs(counts, T, N, K, gated, bias, gather, seed, behind=0):
     offsets = torch.tensor([0] + list(np.cumsum(counts)), dtype=torch.int32)
     R = int(offsets[-1]) + behind
     rows = torch.randint(0, T, (R,), generator=gen, dtype=torch.int32) if gather else None
-    x = torch.randn(T if gather else R, K, generator=gen).half()
+    x = rows_of_x(gen, T if gather else R, K, coarse)
     b = torch.randn(E, n2, generator=gen).to(bias) if bias else None
     return x, codes, grid, offsets, rows, b
 

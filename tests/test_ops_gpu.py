@@ -18,7 +18,15 @@ def dev(*ts):
     return [t.to(DEV) if t is not None else None for t in ts]
 
 
-@pytest.fixture(params=[-1, 1, 2, 3], ids=["auto", "rows", "gemm", "split"])
+@pytest.fixture(autouse=True)
+def sixteen_bit_operands():
+    """Sums of exact products unless a test asks for 8-bit operands."""
+    before = capi.lib().dmm_set_gemv_8bit(0)
+    yield
+    capi.lib().dmm_set_gemv_8bit(before)
+
+
+@pytest.fixture(params=[-1, 1, 2, 3, 4], ids=["auto", "rows", "gemm", "split", "rows8"])
 def kernel(request):
     """The library's choice, and every kernel in its place where it can take the call."""
     lib = capi.lib()
@@ -27,8 +35,8 @@ def kernel(request):
     lib.dmm_set_ops_kernel(-1)
 
 
-def check_fused(M, N, K, gated=False, act="none", bias=None, residual=None, out=F16, seed=0, fp8=True, scale=None):
-    x, codes, grid, b, r = fused_inputs(M, N, K, gated, bias, residual, seed + M + N + K, fp8=fp8)
+def check_fused(M, N, K, gated=False, act="none", bias=None, residual=None, out=F16, seed=0, fp8=True, scale=None, kernel=-1):
+    x, codes, grid, b, r = fused_inputs(M, N, K, gated, bias, residual, seed + M + N + K, fp8=fp8, coarse=kernel == 4)
     s = 1.0 / math.sqrt(max(K, 1)) if scale is None else scale
     xd, cd, gd, bd, rd = dev(x, codes, grid, b, r)
     y = dmm.decode_matmul_fused(xd, cd, gd, s, bias=bd, activation=act, gated=gated, residual=rd, out_dtype=out)
@@ -50,15 +58,15 @@ def test_fused_any_shape(M, N, K, gated):
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("bias,residual,out", [(None, None, F16), (F16, F32, F16), (F32, F16, F32), (None, F16, F16)])
 def test_fused_epilogues(act, gated, bias, residual, out, kernel):
-    check_fused(1, 272, 512, gated, act, bias, residual, out)
-    check_fused(7, 272, 512, gated, act, bias, residual, out)
-    check_fused(40, 272, 512, gated, act, bias, residual, out)
+    check_fused(1, 272, 512, gated, act, bias, residual, out, kernel=kernel)
+    check_fused(7, 272, 512, gated, act, bias, residual, out, kernel=kernel)
+    check_fused(40, 272, 512, gated, act, bias, residual, out, kernel=kernel)
 
 
 @pytest.mark.parametrize("M", [1, 2, 4, 5, 8, 9, 16, 17, 31, 32, 33, 64, 65, 100, 129, 300])
 @pytest.mark.parametrize("N,K,gated", [(64, 256, False), (100, 768, True), (17, 320, False), (1030, 1024, True), (515, 2112, False)])
 def test_fused_rows(M, N, K, gated, kernel):
-    check_fused(M, N, K, gated, "gelu_tanh", F16, None, F16)
+    check_fused(M, N, K, gated, "gelu_tanh", F16, None, F16, kernel=kernel)
 
 
 def test_fused_gate_and_up_scales():
@@ -67,14 +75,54 @@ def test_fused_gate_and_up_scales():
 
 
 @pytest.mark.parametrize("M", [1, 3, 40])
-def test_fused_grid_that_does_not_fit_8_bits(M):
+def test_fused_grid_that_does_not_fit_8_bits(M, kernel):
     check_fused(M, 4240, 512, False, "relu", F16, F16, F16, fp8=False)
     check_fused(M, 2128, 512, True, "silu", F16, F16, F16, fp8=False)
+    check_fused(M, 40000, 256, False, "none", None, None, F16, fp8=False)
+
+
+@pytest.mark.parametrize("M,N,K,gated", [(1, 4096, 4096, False), (2, 4128, 11008, False), (1, 5504, 4096, True), (2, 40004, 512, False),
+                                         (1, 20000, 512, True), (2, 8200, 320, True), (1, 16400, 8192, False)])
+@pytest.mark.parametrize("coarse", [True, False])
+def test_fused_on_8_bit_operands(M, N, K, gated, coarse):
+    """The library's own choice for one or two rows: the exact products' bound where every sum is exact on 8-bit operands
+    too, the plain product's tolerance on them (1e-2 of z and of its unit) for normal x."""
+    capi.lib().dmm_set_gemv_8bit(1)
+    x, codes, grid, b, r = fused_inputs(M, N, K, gated, F16, F16, M + N + K, coarse=coarse)
+    s = 1.0 / math.sqrt(K)
+    xd, cd, gd, bd, rd = dev(x, codes, grid, b, r)
+    y = dmm.decode_matmul_fused(xd, cd, gd, s, bias=bd, activation="silu" if gated else "none", gated=gated, residual=rd)
+    want, tol = product64(x.double(), decode64(codes, grid), (s, s), b, gated, "silu" if gated else "none", r, F16)
+    if not coarse:
+        z = (x.double() @ decode64(codes, grid).t() * s + b.double()).abs()
+        e = 1e-2 * (1 + z)
+        tol = tol + (1.13 * e[:, :N] * (z[:, N:] + e[:, N:]) + z[:, :N] * e[:, N:] if gated else e)
+    assert_within(y, want, tol)
+
+
+def test_grouped_on_8_bit_operands_and_x_that_is_not_finite():
+    """Many jobs per workgroup, some with an infinity: those rows, and no others, are not finite."""
+    capi.lib().dmm_set_gemv_8bit(1)
+    capi.lib().dmm_set_ops_kernel(4)
+    try:
+        for gated in (False, True):
+            counts = (1, 0, 2, 3, 1)
+            x, codes, grid, offsets, rows, b = grouped_inputs(counts, 4, 9000, 768, gated, F16, True, 5, coarse=True)
+            x[2, 700] = math.inf
+            rows[:7] = torch.tensor([0, 1, 2, 3, 2, 0, 1], dtype=torch.int32)
+            y = dmm.decode_matmul_grouped(*dev(x, codes, grid), 0.03, offsets.to(DEV), rows=rows.to(DEV), bias=b.to(DEV), gated=gated)
+            want, tol = grouped64(x, codes, grid, 0.03, offsets, rows, b, gated, "none", F16, 9000)
+            bad = rows == 2
+            assert_within(y[~bad.to(DEV)], want[~bad], tol[~bad])
+            assert not torch.isfinite(y[bad.to(DEV)]).any()
+            assert torch.equal(torch.isnan(y[bad.to(DEV)]).cpu(), torch.isnan(want[bad]))
+    finally:
+        capi.lib().dmm_set_ops_kernel(-1)
 
 
 @pytest.mark.parametrize("M", [1, 4, 16, 40])
 def test_fused_x_that_is_not_finite_stays_in_its_row(M, kernel):
-    x, codes, grid, _, _ = fused_inputs(M, 4240, 512, False, None, None, seed=5)
+    x, codes, grid, _, _ = fused_inputs(M, 4240, 512, False, None, None, seed=5, coarse=kernel == 4)
     x[M - 1, 500] = math.inf
     y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.05)
     want, tol = product64(x.double(), decode64(codes, grid), (0.05, 0.05), None, False, "none", None, F16)
@@ -128,8 +176,9 @@ def test_fused_buffers_at_odd_places(M, N, K):
 
 
 # ----------------------------------------------------------------- by expert
-def check_grouped(counts, T, N, K, gated=False, act="none", bias=None, gather=True, behind=0, out=F16, scale=None, seed=0):
-    x, codes, grid, offsets, rows, b = grouped_inputs(counts, T, N, K, gated, bias, gather, seed + N + K, behind)
+def check_grouped(counts, T, N, K, gated=False, act="none", bias=None, gather=True, behind=0, out=F16, scale=None, seed=0,
+                  kernel=-1):
+    x, codes, grid, offsets, rows, b = grouped_inputs(counts, T, N, K, gated, bias, gather, seed + N + K, behind, coarse=kernel == 4)
     s = 1.0 / math.sqrt(K) if scale is None else scale
     R = x.shape[0] if rows is None else rows.shape[0]
     y = torch.full((R, N), math.nan, dtype=out, device=DEV)
@@ -147,26 +196,26 @@ COUNTS = [(1,), (0, 1), (3, 0, 0, 4, 1), (0, 0, 0), (17, 1, 0, 33, 5, 16), (1,) 
 @pytest.mark.parametrize("counts", COUNTS)
 @pytest.mark.parametrize("N,K,gated", [(64, 256, False), (36, 512, True), (21, 320, False), (272, 1024, True)])
 def test_grouped(counts, N, K, gated, kernel):
-    check_grouped(counts, 11, N, K, gated, "silu" if gated else "none", F16 if gated else None, gather=True, behind=3)
+    check_grouped(counts, 11, N, K, gated, "silu" if gated else "none", F16 if gated else None, gather=True, behind=3, kernel=kernel)
 
 
 @pytest.mark.parametrize("counts", [(3, 0, 0, 4, 1), (40, 0, 25)])
 @pytest.mark.parametrize("K", [8, 24, 264, 64, 4096])
 def test_grouped_row_order_and_types(counts, K, kernel):
     E = len(counts)
-    check_grouped(counts, 5, 20, K, False, "gelu", F32, gather=False, behind=1, out=F32, scale=torch.linspace(0.02, 0.05, E))
-    check_grouped(counts, 5, 20, K, True, "relu", F16, gather=True, out=F32, scale=torch.linspace(0.02, 0.05, 2 * E).view(E, 2))
+    check_grouped(counts, 5, 20, K, False, "gelu", F32, gather=False, behind=1, out=F32, scale=torch.linspace(0.02, 0.05, E), kernel=kernel)
+    check_grouped(counts, 5, 20, K, True, "relu", F16, gather=True, out=F32, scale=torch.linspace(0.02, 0.05, 2 * E).view(E, 2), kernel=kernel)
 
 
 def test_grouped_many_tiles_per_workgroup(kernel):
-    check_grouped((2, 0, 1, 19), 9, 8200, 256, False, "none", None)
-    check_grouped((2, 0, 1, 19), 9, 4100, 512, True, "silu", None)
-    check_grouped((1,), 3, 33000, 256, False, "none", None)
+    check_grouped((2, 0, 1, 19), 9, 8200, 256, False, "none", None, kernel=kernel)
+    check_grouped((2, 0, 1, 19), 9, 4100, 512, True, "silu", None, kernel=kernel)
+    check_grouped((1,), 3, 33000, 256, False, "none", None, kernel=kernel)
 
 
 def test_grouped_lists_that_lead_out_of_the_buffers(kernel):
     for counts in ((2, 3), (90, 60)):
-        x, codes, grid, offsets, rows, _ = grouped_inputs(counts, 4, 64, 256, False, None, True, seed=3)
+        x, codes, grid, offsets, rows, _ = grouped_inputs(counts, 4, 64, 256, False, None, True, seed=3, coarse=kernel == 4)
         R = rows.shape[0]
         rows[1], rows[R - 1] = -7, 4                               # outside x: rows of zeros
         xd, cd, gd, od, rd = dev(x, codes, grid, offsets, rows)
