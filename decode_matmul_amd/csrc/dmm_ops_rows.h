@@ -139,13 +139,21 @@ __device__ __forceinline__ const_rows_args_t *rows_args_late()
     return reinterpret_cast<const_rows_args_t *>((uintptr_t)p);
 }
 
+__device__ __forceinline__ OpsRowsArgs rows_args_copy()
+{
+    OpsRowsArgs a;
+    __builtin_memcpy(&a, rows_args_late(), sizeof(a));
+    return a;
+}
+
 // ---- 8-bit operands (gemv_q8d_kernel's arithmetic) for segments of up to two rows.  The sixteen columns of the
 // matrix unit hold four terms of each row (column 4 m + t is term t of row m, of weight 8^-t), the means of the shift
 // term ride in columns 4 m and 4 m + 1.  A wave splits the 256 k of its own step into terms - a lane has one piece
 // of eight, lanes 32 .. 63 those of the second row - and leaves them in its own piece of LDS: term row 4 m + t at a
 // pitch of 272 bytes, the means behind them at a pitch of 80; no barrier, no roles.  What does not fit is found, not
-// computed: a grid fp8 cannot hold sends the workgroup to the 16-bit body before it starts, a row of x that is
-// not finite sends the job, at its end, through rows_job_slow.
+// computed, and left to the 16-bit body in the same launch, with the same jobs: all of them if the grid does not fit
+// fp8 (known before the first), and those that met an x that is not finite (the terms of an infinity mean
+// nothing), which store nothing here.
 constexpr int kO8TermPitch = 272, kO8MeanPitch = 80;
 constexpr int kO8Means = 8 * kO8TermPitch;
 constexpr int kO8Piece = kO8Means + 4 * kO8MeanPitch + 64;   // 2560
@@ -153,52 +161,15 @@ constexpr int kO8Flags = kSTablesBytes + 16 * kO8Piece;      // 16 votes, 2 word
 constexpr int kO8Bytes = kO8Flags + 128 + 64;
 static_assert(kO8Bytes <= 160 * 1024, "tables and pieces have to fit the LDS");
 
-// A job's outputs one by one, weights decoded from the grid in memory, dot products on the vector ALU: what a job whose
-// x is not finite gets (the terms of an infinity mean nothing).  Any x, the 16-bit kernels' arithmetic.
-template <bool kGated, int W>
-__device__ __forceinline__ void rows_job_slow(const OpsRowsArgs &a, const Epi &epi, int expert, int row, int row_end, int unit, int n, int wave,
-                                           int lane)
-{
-    constexpr int kH = kGated ? 2 : 1;
-    const int kc = a.K >> 3;
-    const uint16_t *ce = a.codes + (int64_t)expert * kH * epi.N * kc;
-    const EpiScale sc = epi_scale(epi, expert);
-    for (int i = wave; i < n * 16; i += W) {
-        const int col = unit * 16 + i;
-        if (col >= epi.N) break;
-        for (int m = row; m < row_end; m++) {
-            const int t = group_row(a.g, m);
-            float acc[kH] = {};
-            for (int j = lane; j < kc; j += kWave) {
-                const uint16_t *xp = a.x + (int64_t)(t < 0 ? 0 : t) * a.K + j * 8;
-#pragma unroll
-                for (int h = 0; h < kH; h++) {
-                    const uint32_t c = ce[((int64_t)col + (int64_t)h * epi.N) * kc + j];
-                    const u4_t gr = reinterpret_cast<const u4_t *>(a.grid)[c & 0xFFu], sr = sign_row((c >> 8) & 0x7Fu);
-                    const h2_t d = as_h2(((c & 0x8000u) * 0x10001u) | 0x34003400u);
-#pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        const h2_t w = __builtin_elementwise_fma(as_h2(gr[p]), as_h2(sr[p]), d);
-                        const float x0 = t < 0 ? 0.f : (float)__builtin_bit_cast(half_t, xp[2 * p]);
-                        const float x1 = t < 0 ? 0.f : (float)__builtin_bit_cast(half_t, xp[2 * p + 1]);
-                        acc[h] = __builtin_fmaf(x1, (float)w[1], __builtin_fmaf(x0, (float)w[0], acc[h]));
-                    }
-                }
-            }
-            const float v = wave_sum(acc[0]), u = kGated ? wave_sum(acc[kH - 1]) : 0.f;
-            if (lane == 0) epi_store1<kGated>(epi, sc, v, u, m, col, expert);
-        }
-    }
-}
-
 // XI, W, CG as in gemv_f16d_kernel: 2 XI rows of x per group, W waves, CG groups of sixteen rows per segment; SR: rows of
 // a segment, CG * 2 XI or fewer.
 // kOne: a dense call of one segment whose workgroups have one job each (up to NU units): the range comes from the
 // host, rows of x follow each other, and the loop has only chunks to count (11008 -> 4096 with one row: 8.1 us as a
 // job of the general form, 6.8 like this).
-// kQ8: 8-bit operands, XI = 1; false if the grid does not fit them and nothing was done.
-template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne, int SR, bool kQ8>
-__device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
+// kQ8: 8-bit operands, XI = 1.
+// todo: the jobs to do, one bit each, the last bit for all from there on (kSome; otherwise all).  Returns the jobs left to do.
+template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne, int SR, bool kQ8, bool kSome>
+__device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint32_t todo)
 {
     const uint16_t *__restrict__ x = args.x;
     const uint16_t *__restrict__ codes = args.codes;
@@ -239,7 +210,7 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
         cur.left = args.units_q + (b < args.units_r ? 1 : 0);
         cur.row_end = g.R;
     } else {
-        if (!ops_range<SR, NU>(g, upn, lane, cur)) return true;   // the whole workgroup, before any barrier
+        if (!ops_range<SR, NU>(g, upn, lane, cur)) return 0u;   // the whole workgroup, before any barrier
         cur = OpsCursor{uniform(cur.expert), uniform(cur.row), uniform(cur.row_end), uniform(cur.unit), uniform(cur.left), uniform(cur.per)};
     }
 
@@ -355,27 +326,43 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
         __builtin_amdgcn_sched_barrier(0);
         stream_stage_grid<64 * W>(smem_raw, grow, tid);
     }
+    // kQ8: the slice of x that has arrived into terms and means, in the wave's piece: for the first item beside the other
+    // waves' tables, for the others behind the tiles of the item before
+    bool finite = true;   // the x of this wave's steps of the job, so far
+    auto split_x = [&]() {
+        u2_t tm[4];
+        uint32_t mean;
+        finite = finite & qd_split_piece(xv[0][0], tm, mean);
+        const uint32_t m = (uint32_t)lane >> 5, pc = (uint32_t)lane & 31;
+        typedef __attribute__((address_space(3))) u2_t lds_u2_rw_t;
+        typedef __attribute__((address_space(3))) uint16_t lds_u16_rw_t;
+#pragma unroll
+        for (int t = 0; t < 4; t++) *reinterpret_cast<lds_u2_rw_t *>(piece + (m * 4 + t) * kO8TermPitch + pc * 8) = tm[t];
+        *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + m * 2 * kO8MeanPitch + pc * 2) = (uint16_t)mean;
+        *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + (m * 2 + 1) * kO8MeanPitch + pc * 2) = (uint16_t)(mean >> 16);
+    };
+    if constexpr (kQ8) split_x();
 #pragma unroll
     for (int d = 1; d < D; d++) issue(cw[d], it, d);
     __syncthreads();
     if constexpr (kQ8) {
         if (__builtin_amdgcn_ballot_w64(flags[lane & 15] != 0) != 0) {
             __syncthreads();   // everybody has read the votes: the other body may have the LDS
-            return false;
+            return ~0u;
         }
     }
     // kQ8: this lane's column of the two B operands and of the means inside the piece; idle columns read the zeros
     const uint32_t zeros = lds_addr(smem_raw) + (uint32_t)(kO8Flags + 128);
     const uint32_t o8_t = c16 < 8 ? piece + (uint32_t)(c16 * kO8TermPitch + q * 64) : zeros;
     const uint32_t o8_m = c16 < 8 && (c16 & 3) < 2 ? piece + (uint32_t)(kO8Means + ((c16 >> 2) * 2 + (c16 & 1)) * kO8MeanPitch + q * 16) : zeros;
-    bool finite = true;   // kQ8: the x of this wave's steps of the job, so far
-    int parity = 0;       // of the job
 
     f4_t acc[NT][CG];
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
         for (int gi = 0; gi < CG; gi++) acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
+    int job = 0;
+    uint32_t left = 0;   // kQ8: jobs that met an x that is not finite
 
     while (kOne ? it.chunk < n_chunks : it.n > 0) {
         // (a value of its own every time round: what depends on it is not kept in scalar registers through the loop)
@@ -387,16 +374,6 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
         i8_t xb0{}, xb1{};
         h8_t xm{};
         if constexpr (kQ8) {
-            u2_t tm[4];
-            uint32_t mean;
-            finite = finite & qd_split_piece(xv[0][0], tm, mean);
-            const uint32_t m = (uint32_t)lane >> 5, pc = (uint32_t)lane & 31;
-            typedef __attribute__((address_space(3))) u2_t lds_u2_rw_t;
-            typedef __attribute__((address_space(3))) uint16_t lds_u16_rw_t;
-#pragma unroll
-            for (int t = 0; t < 4; t++) *reinterpret_cast<lds_u2_rw_t *>(piece + (m * 4 + t) * kO8TermPitch + pc * 8) = tm[t];
-            *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + m * 2 * kO8MeanPitch + pc * 2) = (uint16_t)mean;
-            *reinterpret_cast<lds_u16_rw_t *>(piece + kO8Means + (m * 2 + 1) * kO8MeanPitch + pc * 2) = (uint16_t)(mean >> 16);
             const u4_t r0 = lds_read16(o8_t), r1 = lds_read16(o8_t + 16), r2 = lds_read16(o8_t + 32), r3 = lds_read16(o8_t + 48);
             xm = __builtin_bit_cast(h8_t, lds_read16(o8_m));
             xb0 = i8_t{(int)r0[0], (int)r0[1], (int)r0[2], (int)r0[3], (int)r1[0], (int)r1[1], (int)r1[2], (int)r1[3]};
@@ -423,21 +400,7 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
         }
         if (it.chunk + 1 == n_chunks) {
             // the end of a job: cell (tile, quarter, column) of every wave's piece, a group of rows at a time
-            const const_rows_args_t *late = rows_args_late();
-            Epi epi;
-            epi.bias = late->epi.bias;
-            epi.residual = late->epi.residual;
-            epi.y = late->epi.y;
-            epi.scales = late->epi.scales;
-            epi.scale = late->epi.scale;
-            epi.scale_up = late->epi.scale_up;
-            epi.N = late->epi.N;
-            epi.act = late->epi.act;
-            epi.scale_cols = late->epi.scale_cols;
-            epi.bias_f32 = late->epi.bias_f32;
-            epi.residual_f32 = late->epi.residual_f32;
-            epi.out_f32 = late->epi.out_f32;
-            epi.vec = late->epi.vec;
+            const Epi epi = rows_args_copy().epi;
             const EpiScale sc = epi_scale(epi, it.expert);
 #pragma unroll
             for (int gi = 0; gi < CG; gi++) {
@@ -462,20 +425,20 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
                     acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
                 }
                 if constexpr (kQ8) {
-                    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && lane == 0) flags[16 + parity] = 1u;
+                    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && lane == 0) flags[16 + (job & 1)] = 1u;
                     finite = true;
                 }
                 __syncthreads();
+                bool store = true;
                 if constexpr (kQ8) {
-                    const bool slow = __builtin_amdgcn_ballot_w64(flags[16 + parity] != 0) != 0;
-                    parity ^= 1;
-                    if (tid == 0) flags[16 + parity] = 0u;   // read by all before this job's barrier, set again behind the next one
-                    if (slow) {
-                        rows_job_slow<kGated, W>(args, epi, it.expert, it.row, it.row_end, it.unit, it.n, wave, lane);
-                        break;
+                    if (__builtin_amdgcn_ballot_w64(flags[16 + (job & 1)] != 0) != 0) {
+                        left |= 1u << (job < 31 ? job : 31);
+                        store = false;
                     }
+                    if (tid == 0) flags[17 - (job & 1)] = 0u;   // read by all before this job's barrier, set again behind the next one
                 }
-                for (int cell = tid; cell < it.n * 4 * CM; cell += 64 * W) {
+                if constexpr (kSome) store = (todo >> (job < 31 ? job : 31) & 1u) != 0;
+                for (int cell = tid; store && cell < it.n * 4 * CM; cell += 64 * W) {
                     const int u = cell / (4 * CM), rem = cell % (4 * CM);
                     const int m = it.row + gi * CM + rem % CM;
                     if (m >= it.row_end) continue;
@@ -490,21 +453,31 @@ __device__ __forceinline__ bool ops_rows_body(const OpsRowsArgs &args)
                     epi_store4<kGated, (W == 16)>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
                 }
             }
+            job++;
             if constexpr (!kOne) __syncthreads();   // the pieces take the x of the next job next
+        }
+        if constexpr (kQ8) {
+            if (!kOne || nx.chunk < n_chunks) split_x();
         }
         it = nx;
     }
-    return true;
+    if constexpr (kQ8) {
+        if (left != 0) __syncthreads();   // the other body may have the LDS
+    }
+    return left;
 }
 
 template <int NT, int D, int XI, int W, int CG, bool kGated, bool kOne>
 __global__ __launch_bounds__(64 * W) void ops_rows_kernel(OpsRowsArgs args)
 {
-    ops_rows_body<NT, D, XI, W, CG, kGated, kOne, 2 * XI * CG, false>(args);
+    ops_rows_body<NT, D, XI, W, CG, kGated, kOne, 2 * XI * CG, false, false>(args, ~0u);
 }
 
 template <int NT, int D, bool kGated, bool kOne>
 __global__ __launch_bounds__(1024) void ops_rows8_kernel(OpsRowsArgs args)
 {
-    if (!ops_rows_body<NT, D, 1, 16, 1, kGated, kOne, 2, true>(args)) ops_rows_body<NT, D, 2, 16, 1, kGated, kOne, 2, false>(args);
+    const uint32_t left = ops_rows_body<NT, D, 1, 16, 1, kGated, kOne, 2, true, false>(args, ~0u);
+    if (left == 0) return;
+    const OpsRowsArgs again = rows_args_copy();   // not held in registers meanwhile
+    ops_rows_body<NT, D, 2, 16, 1, kGated, kOne, 2, false, true>(again, left);
 }
