@@ -33,16 +33,16 @@ __device__ __forceinline__ void lds_write16(uint32_t byte_addr, const u4_t &v)
     *reinterpret_cast<lds_u4_rw_t *>(byte_addr) = v;
 }
 
-// w = g * s + d with d taken from the low (kHi = false) or high half of dd for both lanes
+// w = g * s + d with d taken from the low (kHi = false) or high half of dd for both lanes: one v_pk_fma_f16, the
+// broadcast in its op_sel bits.  Plain code, not inline assembly: the results go into registers that a matrix
+// instruction may still be reading as its C operand, and the compiler only keeps the distance the hardware asks for
+// (three wait states behind a 16x16x32) from instructions that it knows to be vector ones.
 template <bool kHi>
 __device__ __forceinline__ uint32_t pk_fma_bcast(uint32_t g, uint32_t s, uint32_t dd)
 {
-    uint32_t r;
-    if (kHi)
-        asm("v_pk_fma_f16 %0, %1, %2, %3 op_sel:[0,0,1] op_sel_hi:[1,1,1]" : "=v"(r) : "v"(g), "v"(s), "v"(dd));
-    else
-        asm("v_pk_fma_f16 %0, %1, %2, %3 op_sel:[0,0,0] op_sel_hi:[1,1,0]" : "=v"(r) : "v"(g), "v"(s), "v"(dd));
-    return r;
+    const h2_t dv = as_h2(dd);
+    const h2_t d = kHi ? h2_t{dv[1], dv[1]} : h2_t{dv[0], dv[0]};
+    return as_u32(__builtin_elementwise_fma(as_h2(g), as_h2(s), d));
 }
 
 // ------------------------------------------------------------------ streaming matrix-vector path
@@ -114,13 +114,8 @@ __device__ __forceinline__ float row_sum16(float v)
     return dpp_shr_add<0x111>(v);   // row_shr:1
 }
 
-// (a & m) | (b & ~m) in one instruction
-__device__ __forceinline__ uint32_t bfi(uint32_t m, uint32_t a, uint32_t b)
-{
-    uint32_t r;
-    asm("v_bfi_b32 %0, %1, %2, %3" : "=v"(r) : "s"(m), "v"(a), "v"(b));
-    return r;
-}
+// one v_bfi_b32
+__device__ __forceinline__ uint32_t bfi(uint32_t m, uint32_t a, uint32_t b) { return (a & m) | (b & ~m); }
 
 struct StreamGather {
     u4_t g0, s0, g1, s1;
