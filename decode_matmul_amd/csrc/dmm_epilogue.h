@@ -111,25 +111,37 @@ __device__ __forceinline__ f4_t epi_act4(f4_t z, int act)
     return z;
 }
 
-// four outputs (row, n .. n + 3), n % 4 == 0; those past N are left out
-template <bool kGated, bool kSmall>
-__device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n,
-                                           int expert)
+// what the epilogue of four outputs (row, n .. n + 3), n % 4 == 0, reads beside the sums
+struct EpiOperands {
+    f4_t bias, bias_up, residual;
+};
+template <bool kGated>
+__device__ __forceinline__ EpiOperands epi_fetch4(const Epi &e, int64_t row, int n, int expert)
 {
-    if (n >= e.N) return;
-    const int left = e.N - n;   // outputs that exist, from here on
+    const int left = e.N - n;
+    EpiOperands o;
+    o.bias = o.bias_up = o.residual = f4_t{0.f, 0.f, 0.f, 0.f};
+    if (left <= 0) return o;
     const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
-    const int64_t i = row * e.N + n;
-    // every operand is asked for before the first is used
-    f4_t bz = f4_t{0.f, 0.f, 0.f, 0.f}, bu = bz, rs = bz;
     if (e.bias) {
-        bz = epi_load4(e.bias, b, e.bias_f32, e.vec, left);
-        if (kGated) bu = epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
+        o.bias = epi_load4(e.bias, b, e.bias_f32, e.vec, left);
+        if (kGated) o.bias_up = epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
     }
-    if (e.residual) rs = epi_load4(e.residual, i, e.residual_f32, e.vec, left);
-    f4_t z = epi_act4<kSmall>(v * sc.s + bz, e.act);
-    if (kGated) z *= u * sc.up + bu;
-    if (e.residual) z += rs;
+    if (e.residual) o.residual = epi_load4(e.residual, row * e.N + n, e.residual_f32, e.vec, left);
+    return o;
+}
+
+// the four outputs; those past N are left out
+template <bool kGated, bool kSmall>
+__device__ __forceinline__ void epi_finish4(const Epi &e, const EpiScale &sc, const EpiOperands &o, const f4_t &v, const f4_t &u, int64_t row,
+                                            int n)
+{
+    const int left = e.N - n;   // outputs that exist, from here on
+    if (left <= 0) return;
+    const int64_t i = row * e.N + n;
+    f4_t z = epi_act4<kSmall>(v * sc.s + o.bias, e.act);
+    if (kGated) z *= u * sc.up + o.bias_up;
+    if (e.residual) z += o.residual;
     if (!e.vec) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -145,6 +157,12 @@ __device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, con
         for (int k = 0; k < 4; k++) o[k] = (half_t)z[k];
         *reinterpret_cast<h4_t *>(reinterpret_cast<half_t *>(e.y) + i) = o;
     }
+}
+
+template <bool kGated, bool kSmall>
+__device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n, int expert)
+{
+    epi_finish4<kGated, kSmall>(e, sc, epi_fetch4<kGated>(e, row, n, expert), v, u, row, n);
 }
 
 // ------------------------------------------------------------------ rows by expert

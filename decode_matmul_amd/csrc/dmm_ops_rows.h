@@ -401,33 +401,49 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
         if (it.chunk + 1 == n_chunks) {
             // the end of a job: cell (tile, quarter, column) of every wave's piece, a group of rows at a time
             const Epi epi = rows_args_copy().epi;
+            // (the thread's number as a value of its own: addresses made from it are not held through the loop)
+            int jtid = tid;
+            asm volatile("" : "+v"(jtid));
+            const int jl = jtid & 63, jc = jl & 15, jq = jl >> 4;
             const EpiScale sc = epi_scale(epi, it.expert);
 #pragma unroll
             for (int gi = 0; gi < CG; gi++) {
                 if (gi > 0) __syncthreads();   // the readers of the group before are done with the pieces
+                // Sixteen waves: the sixteen lanes of a row add one cell up, a wave's sums each (cell c of wave w lies in slot
+                // c ^ w, so that they meet no bank conflict), and lane 15 has it; the first cell's operands are asked for ahead of the
+                // barrier.  Eight waves of sixteen rows have a cell for every thread: each adds its own up.
+                constexpr bool kLanes = W == 16;
+                const int n_cells = it.n * 4 * CM;
+                auto cell_row = [&](int cell) { return it.row + gi * CM + cell % CM; };
+                auto cell_col = [&](int cell) { return (it.unit + cell / (4 * CM)) * 16 + 4 * (cell % (4 * CM) / CM); };
+                auto cell_live = [&](int cell) { return cell < n_cells && cell_row(cell) < it.row_end; };
+                const int cell0 = kLanes ? jtid >> 4 : jtid;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     if (t < nt) {
                         f4_t v = acc[t][gi];
-                        int col = c16;
+                        int col = jc;
                         if constexpr (kQ8) {   // the four terms of a row, with their weights 8^-t, into the lane of column 4 m
-                            const float wt = __builtin_bit_cast(float, 0x3F800000u - (((uint32_t)c16 & 3u) * 3u << 23));
+                            const float wt = __builtin_bit_cast(float, 0x3F800000u - (((uint32_t)jc & 3u) * 3u << 23));
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 v[e] *= wt;
                                 v[e] = dpp_shl_add<1>(v[e], v[e]);
                                 v[e] = dpp_shl_add<2>(v[e], v[e]);
                             }
-                            col = (c16 & 3) == 0 ? c16 >> 2 : CM;
+                            col = (jc & 3) == 0 ? jc >> 2 : CM;
                         }
-                        if (col < CM) lds_write16(piece + (uint32_t)((t * 4 + q) * CM + col) * 16, __builtin_bit_cast(u4_t, v));
+                        if (col < CM)
+                            lds_write16(piece + (uint32_t)(((t * 4 + jq) * CM + col) ^ (kLanes ? wave : 0)) * 16, __builtin_bit_cast(u4_t, v));
                     }
                     acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
                 }
                 if constexpr (kQ8) {
-                    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && lane == 0) flags[16 + (job & 1)] = 1u;
+                    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && jl == 0) flags[16 + (job & 1)] = 1u;
                     finite = true;
                 }
+                EpiOperands ops0{};
+                if (kLanes && jc == 15 && cell_live(cell0)) ops0 = epi_fetch4<kGated>(epi, cell_row(cell0), cell_col(cell0), it.expert);
                 __syncthreads();
                 bool store = true;
                 if constexpr (kQ8) {
@@ -435,22 +451,40 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
                         left |= 1u << (job < 31 ? job : 31);
                         store = false;
                     }
-                    if (tid == 0) flags[17 - (job & 1)] = 0u;   // read by all before this job's barrier, set again behind the next one
+                    if (jtid == 0) flags[17 - (job & 1)] = 0u;   // read by all before this job's barrier, set again behind the next one
                 }
                 if constexpr (kSome) store = (todo >> (job < 31 ? job : 31) & 1u) != 0;
-                for (int cell = tid; store && cell < it.n * 4 * CM; cell += 64 * W) {
-                    const int u = cell / (4 * CM), rem = cell % (4 * CM);
-                    const int m = it.row + gi * CM + rem % CM;
-                    if (m >= it.row_end) continue;
-                    const uint32_t src = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + ((kGated ? 2 * u : u) * 4 * CM + rem) * 16);
-                    f4_t v = f4_t{0.f, 0.f, 0.f, 0.f}, up = v;
-#pragma unroll kSumUnroll
-                    for (int w = 0; w < W; w++) v += __builtin_bit_cast(f4_t, lds_read16(src + w * kPiece));
-                    if constexpr (kGated) {
-#pragma unroll kSumUnroll
-                        for (int w = 0; w < W; w++) up += __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16 + w * kPiece));
+                const uint32_t sums = lds_addr(smem_raw) + (uint32_t)kSTablesBytes;
+                auto slot_of = [&](int cell) { return kGated ? cell / (4 * CM) * 8 * CM + cell % (4 * CM) : cell; };
+                if constexpr (kLanes) {
+                    for (int c0 = 0; store && c0 < n_cells; c0 += 64) {
+                        const int cell = c0 + cell0, slot = slot_of(cell);
+                        const uint32_t src = sums + (uint32_t)(jc * kPiece);
+                        f4_t v = __builtin_bit_cast(f4_t, lds_read16(src + (uint32_t)((slot ^ jc) << 4))), up = f4_t{0.f, 0.f, 0.f, 0.f};
+                        if constexpr (kGated) up = __builtin_bit_cast(f4_t, lds_read16(src + (uint32_t)(((slot + 4 * CM) ^ jc) << 4)));
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v[e] = row_sum16(v[e]);
+                            if (kGated) up[e] = row_sum16(up[e]);
+                        }
+                        if (jc == 15 && cell_live(cell)) {
+                            if (c0 > 0) ops0 = epi_fetch4<kGated>(epi, cell_row(cell), cell_col(cell), it.expert);
+                            epi_finish4<kGated, true>(epi, sc, ops0, v, up, cell_row(cell), cell_col(cell));
+                        }
                     }
-                    epi_store4<kGated, (W == 16)>(epi, sc, v, up, m, (it.unit + u) * 16 + 4 * (rem / CM), it.expert);
+                } else {
+                    for (int cell = jtid; store && cell < n_cells; cell += 64 * W) {
+                        if (!cell_live(cell)) continue;
+                        const uint32_t src = sums + (uint32_t)(slot_of(cell) * 16);
+                        f4_t v = f4_t{0.f, 0.f, 0.f, 0.f}, up = v;
+#pragma unroll kSumUnroll
+                        for (int w = 0; w < W; w++) v += __builtin_bit_cast(f4_t, lds_read16(src + w * kPiece));
+                        if constexpr (kGated) {
+#pragma unroll kSumUnroll
+                            for (int w = 0; w < W; w++) up += __builtin_bit_cast(f4_t, lds_read16(src + 4 * CM * 16 + w * kPiece));
+                        }
+                        epi_store4<kGated, false>(epi, sc, v, up, cell_row(cell), cell_col(cell), it.expert);
+                    }
                 }
             }
             job++;
