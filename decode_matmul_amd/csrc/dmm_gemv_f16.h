@@ -220,11 +220,11 @@ __device__ __forceinline__ float dpp_shl_add(float v, float w)
 // of the columns that hold no x)
 __host__ __device__ constexpr int64_t stream_x_bytes(int64_t M, int64_t K) { return M * (2 * K + 16) + 128; }
 
-template <int R, int W, int D, bool kPacked, int JP>
-__device__ __forceinline__ void gemv_stream_body(const uint16_t *__restrict__ x, const uint16_t *__restrict__ codes,
-                                                 const void *__restrict__ grid, float scale,
-                                                 uint16_t *__restrict__ y, int M, int N, int K, int tiles_q,
-                                                 int tiles_r)
+// store(m, n, v): what becomes of the sums v of rows n .. n + 3 of W (all below N) with row m of x
+template <int R, int W, int D, bool kPacked, int JP, class Store>
+__device__ __forceinline__ void gemv_stream_body_to(const uint16_t *__restrict__ x, const uint16_t *__restrict__ codes,
+                                                    const void *__restrict__ grid, const Store &store, int M, int N, int K,
+                                                    int tiles_q, int tiles_r)
 {
     static_assert(R == 1 || R == 2, "a partial row block is handled as one tile");
     extern __shared__ __attribute__((aligned(256))) unsigned char smem_raw[];
@@ -384,12 +384,7 @@ __device__ __forceinline__ void gemv_stream_body(const uint16_t *__restrict__ x,
             for (int e = 0; e < 4; e++) v[e] = row_sum16(v[e]);
             const int tile = t0 + blk * R + r;
             const int n = tile * 16 + 4 * q;
-            if (c16 == 15 && tile < t1 && n < N) {   // N % 4 == 0, so the four rows are in range together
-                h4_t o;
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[e] = (half_t)(v[e] * scale);
-                *reinterpret_cast<h4_t *>(y + (int64_t)m * N + n) = o;
-            }
+            if (c16 == 15 && tile < t1 && n < N) store(m, n, v);   // N % 4 == 0, so the four rows are in range together
         }
     };
 
@@ -418,6 +413,22 @@ __device__ __forceinline__ void gemv_stream_body(const uint16_t *__restrict__ x,
             issue(cw[d]);
         }
     }
+}
+
+// y = half(scale * sum)
+template <int R, int W, int D, bool kPacked, int JP>
+__device__ __forceinline__ void gemv_stream_body(const uint16_t *__restrict__ x, const uint16_t *__restrict__ codes,
+                                                 const void *__restrict__ grid, float scale,
+                                                 uint16_t *__restrict__ y, int M, int N, int K, int tiles_q,
+                                                 int tiles_r)
+{
+    auto store = [&](int m, int n, const f4_t &v) {
+        h4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = (half_t)(v[e] * scale);
+        *reinterpret_cast<h4_t *>(y + (int64_t)m * N + n) = o;
+    };
+    gemv_stream_body_to<R, W, D, kPacked, JP>(x, codes, grid, store, M, N, K, tiles_q, tiles_r);
 }
 
 template <int R, int W, int D, bool kPacked, int JP>

@@ -139,6 +139,15 @@ int run_ops_rows8(const void *x, const void *codes, const void *grid, const Grou
     return launch_ops_rows8_inst<8, kGated, false>(x, codes, grid, g, e, K, units, s);
 }
 
+inline int64_t ops_stream_lds(int64_t K) { return (int64_t)kSTablesBytes + stream_red_bytes(1, 16, 1) + stream_x_bytes(1, K); }
+
+int launch_ops_stream(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t tiles = ((int64_t)e.N + 15) / 16;   // one per workgroup
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, 1, 0};
+    return launch(ops_stream_kernel, dim3((unsigned)tiles), dim3(1024), (size_t)ops_stream_lds(K), s, args);
+}
+
 // rows of a segment by the rows an expert has
 template <bool kGated>
 int run_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
@@ -158,6 +167,9 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
     if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
     const bool rows_ok = ops_segments(g, 2) * ((e.N + 15) / 16) < (1LL << 31);
+    if (!kGated && force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0 && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cu_count() &&
+        ops_stream_lds(K) <= kLdsMax)
+        return launch_ops_stream(x, codes, grid, g, e, K, s);
     // 8-bit operands: a job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored
     // twice, which a residual that is the output itself would not survive
     const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 31LL * 16 * 2 * cu_count());
@@ -219,7 +231,7 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_ROUTE(1, 16), DMM_K_ROUTE(2, 16), DMM_K_ROUTE(4, 16), DMM_K_ROUTE(8, 16), DMM_K_ROUTE(16, 16),
         DMM_K_ROUTE(1, 64), DMM_K_ROUTE(2, 64), DMM_K_ROUTE(4, 64), DMM_K_ROUTE(8, 64), DMM_K_ROUTE(16, 64),
 #undef DMM_K_ROUTE
-        kinfo(route_place_kernel, kLdsMax, false),
+        kinfo(route_place_kernel, kLdsMax, false), kinfo(ops_stream_kernel, kLdsMax, true),
     };
     return t;
 }
