@@ -83,12 +83,15 @@ __device__ __forceinline__ void qd_tile_step(const u4_t &cw, uint32_t lane_base,
     }
 }
 
-template <int NT, int U, int D, bool kPacked>
-__global__ __launch_bounds__(1024) void gemv_q8d_kernel(const uint16_t *__restrict__ x,
-                                                        const uint16_t *__restrict__ codes,
-                                                        const void *__restrict__ grid, float scale,
-                                                        uint16_t *__restrict__ y, int N, int K, int tiles_q, int tiles_r)
+// The body serves the operators of dmm_ops.hip too.  What differs is P: whether tiles come in pairs, 16 rows of W and the
+// 16 rows `half` rows further on (P::kPairs; then tiles_q and tiles_r count pairs, NT counts tiles), what becomes of
+// the sums - p.store(n, v), with p.store(n, v, u) for a pair: v the sums of rows n .. n + 3, u those of n + half .. -
+// and who takes a launch that 8-bit operands cannot do, p.hand_over().  N: outputs (rows of W, or of one half).
+template <int NT, int U, int D, bool kPacked, class P>
+__device__ __forceinline__ void gemv_q8d_body(const P &p, const uint16_t *__restrict__ x, const uint16_t *__restrict__ codes,
+                                              const void *__restrict__ grid, int N, int K, int tiles_q, int tiles_r)
 {
+    static_assert(!(P::kPairs && (kPacked || NT % 2 != 0)), "pairs of row-major tiles");
     constexpr int W = 16;
     static_assert((U * NT) % D == 0, "the ring has to divide the unrolled loop");
     extern __shared__ __attribute__((aligned(256))) unsigned char smem_raw[];
@@ -118,11 +121,11 @@ __global__ __launch_bounds__(1024) void gemv_q8d_kernel(const uint16_t *__restri
     u4_t xpiece = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, sp * 16, wave < 8 ? 0 : kOut, 0);
 
     const int t0 = (int)blockIdx.x * tiles_q + ((int)blockIdx.x < tiles_r ? (int)blockIdx.x : tiles_r);
-    const int nt = tiles_q + ((int)blockIdx.x < tiles_r ? 1 : 0);   // <= NT (the host's business)
+    const int nt = (tiles_q + ((int)blockIdx.x < tiles_r ? 1 : 0)) * (P::kPairs ? 2 : 1);   // <= NT (the host's business)
 
     const int n_tiles_all = (N + 15) >> 4;
     const __amdgpu_buffer_rsrc_t crsrc = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t *>(codes), 0, (int)((int64_t)(kPacked ? n_tiles_all * 16 : N) * row_bytes), 0x00020000);
+        const_cast<uint16_t *>(codes), 0, (int)((int64_t)(kPacked ? n_tiles_all * 16 : P::kPairs ? 2 * N : N) * row_bytes), 0x00020000);
     const int voff = kPacked ? lane * 16 : c16 * row_bytes + q * 16;
     const int tile_stride = kPacked ? n_steps * 1024 : 16 * row_bytes;
     const int step_stride = kPacked ? 1024 : 64;
@@ -131,7 +134,8 @@ __global__ __launch_bounds__(1024) void gemv_q8d_kernel(const uint16_t *__restri
     auto issue = [&](u4_t &cwd, int c, int t) {
         const int step = c * W + wave;
         const bool ok = t < nt && step < n_steps;
-        cwd = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? tile0_off + t * tile_stride + step * step_stride : kOut, 0);
+        const int toff = P::kPairs ? (t >> 1) * tile_stride + (t & 1) * N * row_bytes : t * tile_stride;
+        cwd = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? tile0_off + toff + step * step_stride : kOut, 0);
     };
     u4_t cw[D];
     // The first items of the code stream.  The memory pipeline of a compute unit takes a row-major code
@@ -242,25 +246,60 @@ __global__ __launch_bounds__(1024) void gemv_q8d_kernel(const uint16_t *__restri
     }
     __syncthreads();   // the launch's closing barrier: every partial sum is there (or everybody has read the flags)
     if (hand_over) {
-        gemv_stream_body<1, W, 2, kPacked, 4>(x, codes, grid, scale, y, 1, N, K, tiles_q, tiles_r);
+        p.hand_over();
         return;
     }
-    if (wave < nt) {
-        // wave t adds up tile t: lane (w, quarter) takes wave w's 4 columns with their weights 8^-c, then
-        // the 16 lanes of a row are added with DPP shifts
-        const uint32_t src = red + (uint32_t)(wave * kQdRedTile + c16 * kQdRedWave + q * 64);
+    // wave t adds up tile t (or pair t): lane (w, quarter) takes wave w's 4 columns with their weights 8^-c, then
+    // the 16 lanes of a row are added with DPP shifts
+    auto tile_sum = [&](int t) {
+        const uint32_t src = red + (uint32_t)(t * kQdRedTile + c16 * kQdRedWave + q * 64);
         f4_t v = __builtin_bit_cast(f4_t, lds_read16(src));
 #pragma unroll
         for (int cc = 1; cc < 4; cc++)
             v += __builtin_bit_cast(f4_t, lds_read16(src + cc * 16)) * __builtin_bit_cast(float, 0x3F800000u - ((uint32_t)cc * 3u << 23));
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] = row_sum16(v[e]);
-        const int n = (t0 + wave) * 16 + 4 * q;
-        if (c16 == 15 && n < N) {   // N % 4 == 0, so the four rows are in range together
-            h4_t o;
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = (half_t)(v[e] * scale);
-            *reinterpret_cast<h4_t *>(y + n) = o;
+        return v;
+    };
+    const int n = (t0 + wave) * 16 + 4 * q;
+    if constexpr (P::kPairs) {
+        if (2 * wave < nt) {
+            const f4_t v = tile_sum(2 * wave), u = tile_sum(2 * wave + 1);
+            if (c16 == 15 && n < N) p.store(n, v, u);
         }
+    } else if (wave < nt) {
+        const f4_t v = tile_sum(wave);
+        if (c16 == 15 && n < N) p.store(n, v);
     }
+}
+
+template <bool kPacked>
+struct Q8dPlain {
+    static constexpr bool kPairs = false;
+    const uint16_t *x, *codes;
+    const void *grid;
+    float scale;
+    uint16_t *y;
+    int N, K, tiles_q, tiles_r;
+    __device__ __forceinline__ void store(int n, const f4_t &v) const   // N % 4 == 0, so the four rows are in range together
+    {
+        h4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = (half_t)(v[e] * scale);
+        *reinterpret_cast<h4_t *>(y + n) = o;
+    }
+    __device__ __forceinline__ void hand_over() const
+    {
+        gemv_stream_body<1, 16, 2, kPacked, 4>(x, codes, grid, scale, y, 1, N, K, tiles_q, tiles_r);
+    }
+};
+
+template <int NT, int U, int D, bool kPacked>
+__global__ __launch_bounds__(1024) void gemv_q8d_kernel(const uint16_t *__restrict__ x,
+                                                        const uint16_t *__restrict__ codes,
+                                                        const void *__restrict__ grid, float scale,
+                                                        uint16_t *__restrict__ y, int N, int K, int tiles_q, int tiles_r)
+{
+    const Q8dPlain<kPacked> p{x, codes, grid, scale, y, N, K, tiles_q, tiles_r};
+    gemv_q8d_body<NT, U, D, kPacked>(p, x, codes, grid, N, K, tiles_q, tiles_r);
 }

@@ -148,6 +148,37 @@ int launch_ops_stream(const void *x, const void *codes, const void *grid, const 
     return launch(ops_stream_kernel, dim3((unsigned)tiles), dim3(1024), (size_t)ops_stream_lds(K), s, args);
 }
 
+template <int NT, int D, bool kGated>
+int launch_ops_q8d_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
+                        hipStream_t s)
+{
+    const int64_t wgs = units < cu_count() ? units : cu_count();
+    const int64_t lds = std::max<int64_t>(qd_lds_bytes(), fd_lds_bytes(2));   // its own, and the 16-bit body's
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, (int)(units / wgs), (int)(units % wgs)};
+    return launch(ops_q8d_kernel<NT, 1, D, kGated>, dim3((unsigned)wgs), dim3(1024), (size_t)lds, s, args);
+}
+
+inline int64_t ops_share(int64_t N, bool gated)   // most tiles a workgroup gets of one row's matrix
+{
+    const int64_t units = (N + 15) / 16, cus = cu_count();
+    return (units + cus - 1) / cus * (gated ? 2 : 1);
+}
+
+template <bool kGated>
+int launch_ops_q8d(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t units = ((int64_t)e.N + 15) / 16;
+    switch (ops_share(e.N, kGated)) {
+        case 1:
+        case 2: return launch_ops_q8d_inst<2, 2, kGated>(x, codes, grid, g, e, K, units, s);
+        case 3:
+        case 4: return launch_ops_q8d_inst<4, 2, kGated>(x, codes, grid, g, e, K, units, s);
+        case 5:
+        case 6: return launch_ops_q8d_inst<6, 3, kGated>(x, codes, grid, g, e, K, units, s);
+        default: return launch_ops_q8d_inst<8, 2, kGated>(x, codes, grid, g, e, K, units, s);
+    }
+}
+
 // rows of a segment by the rows an expert has
 template <bool kGated>
 int run_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
@@ -170,6 +201,8 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     if (!kGated && force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0 && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cu_count() &&
         ops_stream_lds(K) <= kLdsMax)
         return launch_ops_stream(x, codes, grid, g, e, K, s);
+    if (force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0 && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled())
+        return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
     // 8-bit operands: a job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored
     // twice, which a residual that is the output itself would not survive
     const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 31LL * 16 * 2 * cu_count());
@@ -221,6 +254,11 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_ROWS(false, false), DMM_K_ROWS(true, false), DMM_K_ROWS(false, true), DMM_K_ROWS(true, true),
 #undef DMM_K_ROWS
 #undef DMM_K_ROWS_X
+#define DMM_K_OQ8D(G)                                                                                                             \
+    kinfo(ops_q8d_kernel<2, 1, 2, G>, kLdsMax, true), kinfo(ops_q8d_kernel<4, 1, 2, G>, kLdsMax, true),                           \
+        kinfo(ops_q8d_kernel<6, 1, 3, G>, kLdsMax, true), kinfo(ops_q8d_kernel<8, 1, 2, G>, kLdsMax, true)
+        DMM_K_OQ8D(false), DMM_K_OQ8D(true),
+#undef DMM_K_OQ8D
 #define DMM_K_ROWS8(G)                                                                                                            \
     kinfo(ops_rows8_kernel<2, 2, G, true>, kLdsMax, true), kinfo(ops_rows8_kernel<4, 2, G, true>, kLdsMax, true),                 \
         kinfo(ops_rows8_kernel<8, 2, G, true>, kLdsMax, true), kinfo(ops_rows8_kernel<4, 2, G, false>, kLdsMax, true),            \

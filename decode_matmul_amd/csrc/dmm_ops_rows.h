@@ -526,3 +526,29 @@ __global__ __launch_bounds__(1024) void ops_stream_kernel(OpsRowsArgs args)
     auto store = [&](int m, int n, const f4_t &v) { epi_store4<false, true>(epi, sc, v, v, m, n, 0); };
     gemv_stream_body_to<1, 16, 2, false, 4>(args.x, args.codes, args.grid, store, 1, epi.N, args.K, args.units_q, args.units_r);
 }
+
+// One row of x, up to eight tiles per compute unit: the batch-1 kernel's body on 8-bit operands.  Its roles (tables and the
+// split of x in different waves) leave the tables sooner than the jobs' kernel, where every wave splits its own x
+// (graph launches, us: 4096 -> 11008 5.1 / 6.2).  What it cannot do goes to the 16-bit body.
+template <int NT, bool kGated>
+struct Q8dOps {
+    static constexpr bool kPairs = kGated;
+    const OpsRowsArgs &args;
+    __device__ __forceinline__ void store(int n, const f4_t &v) const { store(n, v, v); }
+    __device__ __forceinline__ void store(int n, const f4_t &v, const f4_t &u) const
+    {
+        epi_store4<kGated, true>(args.epi, epi_scale(args.epi, 0), v, u, 0, n, 0);
+    }
+    __device__ __forceinline__ void hand_over() const
+    {
+        const OpsRowsArgs again = rows_args_copy();
+        ops_rows_body<NT, 2, 2, 16, 1, kGated, true, 4, false, false>(again, ~0u);
+    }
+};
+
+template <int NT, int U, int D, bool kGated>
+__global__ __launch_bounds__(1024) void ops_q8d_kernel(OpsRowsArgs args)
+{
+    const Q8dOps<NT < 2 ? 2 : NT, kGated> p{args};
+    gemv_q8d_body<NT, U, D, false>(p, args.x, args.codes, args.grid, args.epi.N, args.K, args.units_q, args.units_r);
+}
