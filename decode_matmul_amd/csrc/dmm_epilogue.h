@@ -47,16 +47,9 @@ __device__ __forceinline__ float epi_load(const void *p, int64_t i, int f32)
     return f32 ? reinterpret_cast<const float *>(p)[i] : (float)reinterpret_cast<const half_t *>(p)[i];
 }
 
-// four elements from i on, one by one (the first `left` of them) unless vec: i % 4 == 0 and p aligned, see Epi::vec
-__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32, int vec, int left)
+// four elements from i on, i % 4 == 0 and p aligned (Epi::vec)
+__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32)
 {
-    if (!vec) {
-        f4_t r = f4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (k < left) r[k] = epi_load(p, i + k, f32);
-        return r;
-    }
     if (f32) return *reinterpret_cast<const f4_t *>(reinterpret_cast<const float *>(p) + i);
     const h4_t h = *reinterpret_cast<const h4_t *>(reinterpret_cast<const half_t *>(p) + i);
     return f4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
@@ -68,7 +61,7 @@ struct EpiScale {
 __device__ __forceinline__ EpiScale epi_scale(const Epi &e, int expert)
 {
     EpiScale r{e.scale, e.scale_up};
-    if (e.scales) {
+    if (__builtin_expect(e.scales != nullptr, 0)) {
         r.s *= e.scales[(int64_t)expert * e.scale_cols];
         r.up *= e.scales[(int64_t)expert * e.scale_cols + e.scale_cols - 1];
     }
@@ -111,58 +104,59 @@ __device__ __forceinline__ f4_t epi_act4(f4_t z, int act)
     return z;
 }
 
-// what the epilogue of four outputs (row, n .. n + 3), n % 4 == 0, reads beside the sums
+// What the epilogue of four outputs (row, n .. n + 3), n % 4 == 0, n < N, reads beside the sums; without Epi::vec nothing,
+// the outputs go one by one then.  A launch meets its epilogue's code cold, a miss for every line that a branch leads
+// to, so the way that calls take is kept short and straight and everything else out of it.
 struct EpiOperands {
     f4_t bias, bias_up, residual;
 };
 template <bool kGated>
 __device__ __forceinline__ EpiOperands epi_fetch4(const Epi &e, int64_t row, int n, int expert)
 {
-    const int left = e.N - n;
     EpiOperands o;
     o.bias = o.bias_up = o.residual = f4_t{0.f, 0.f, 0.f, 0.f};
-    if (left <= 0) return o;
-    const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
-    if (e.bias) {
-        o.bias = epi_load4(e.bias, b, e.bias_f32, e.vec, left);
-        if (kGated) o.bias_up = epi_load4(e.bias, b + e.N, e.bias_f32, e.vec, left);
+    if (e.bias && e.vec) {
+        const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
+        o.bias = epi_load4(e.bias, b, e.bias_f32);
+        if (kGated) o.bias_up = epi_load4(e.bias, b + e.N, e.bias_f32);
     }
-    if (e.residual) o.residual = epi_load4(e.residual, row * e.N + n, e.residual_f32, e.vec, left);
+    if (e.residual && e.vec) o.residual = epi_load4(e.residual, row * e.N + n, e.residual_f32);
     return o;
 }
 
 // the four outputs; those past N are left out
 template <bool kGated, bool kSmall>
-__device__ __forceinline__ void epi_finish4(const Epi &e, const EpiScale &sc, const EpiOperands &o, const f4_t &v, const f4_t &u, int64_t row,
-                                            int n)
+__device__ __forceinline__ void epi_finish4(const Epi &e, const EpiScale &sc, const EpiOperands &o, f4_t v, f4_t u, int64_t row, int n,
+                                            int expert)
 {
-    const int left = e.N - n;   // outputs that exist, from here on
-    if (left <= 0) return;
-    const int64_t i = row * e.N + n;
+    if (__builtin_expect(!e.vec, 0)) {
+#pragma unroll 1
+        for (int i = n; i < n + 4; i++) {   // the sums turned by one element each time: the code once
+            if (i < e.N) epi_store1<kGated>(e, sc, v[0], u[0], row, i, expert);
+            v = f4_t{v[1], v[2], v[3], v[0]};
+            u = f4_t{u[1], u[2], u[3], u[0]};
+        }
+        return;
+    }
     f4_t z = epi_act4<kSmall>(v * sc.s + o.bias, e.act);
     if (kGated) z *= u * sc.up + o.bias_up;
-    if (e.residual) z += o.residual;
-    if (!e.vec) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (k >= left) break;
-            if (e.out_f32) reinterpret_cast<float *>(e.y)[i + k] = z[k];
-            else reinterpret_cast<half_t *>(e.y)[i + k] = (half_t)z[k];
-        }
-    } else if (e.out_f32) {
+    z += o.residual;   // zeros if there is none
+    const int64_t i = row * e.N + n;
+    if (__builtin_expect(e.out_f32, 0)) {
         *reinterpret_cast<f4_t *>(reinterpret_cast<float *>(e.y) + i) = z;
     } else {
-        h4_t o;
+        h4_t h;
 #pragma unroll
-        for (int k = 0; k < 4; k++) o[k] = (half_t)z[k];
-        *reinterpret_cast<h4_t *>(reinterpret_cast<half_t *>(e.y) + i) = o;
+        for (int k = 0; k < 4; k++) h[k] = (half_t)z[k];
+        *reinterpret_cast<h4_t *>(reinterpret_cast<half_t *>(e.y) + i) = h;
     }
 }
 
 template <bool kGated, bool kSmall>
 __device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n, int expert)
 {
-    epi_finish4<kGated, kSmall>(e, sc, epi_fetch4<kGated>(e, row, n, expert), v, u, row, n);
+    if (n >= e.N) return;
+    epi_finish4<kGated, kSmall>(e, sc, epi_fetch4<kGated>(e, row, n, expert), v, u, row, n, expert);
 }
 
 // ------------------------------------------------------------------ rows by expert

@@ -417,7 +417,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
                 const int n_cells = it.n * 4 * CM;
                 auto cell_row = [&](int cell) { return it.row + gi * CM + cell % CM; };
                 auto cell_col = [&](int cell) { return (it.unit + cell / (4 * CM)) * 16 + 4 * (cell % (4 * CM) / CM); };
-                auto cell_live = [&](int cell) { return cell < n_cells && cell_row(cell) < it.row_end; };
+                auto cell_live = [&](int cell) { return cell < n_cells && cell_row(cell) < it.row_end && cell_col(cell) < N; };
                 const int cell0 = kLanes ? jtid >> 4 : jtid;
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
@@ -470,7 +470,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
                         }
                         if (jc == 15 && cell_live(cell)) {
                             if (c0 > 0) ops0 = epi_fetch4<kGated>(epi, cell_row(cell), cell_col(cell), it.expert);
-                            epi_finish4<kGated, true>(epi, sc, ops0, v, up, cell_row(cell), cell_col(cell));
+                            epi_finish4<kGated, true>(epi, sc, ops0, v, up, cell_row(cell), cell_col(cell), it.expert);
                         }
                     }
                 } else {
