@@ -30,14 +30,16 @@ __device__ __forceinline__ float epi_sigmoid(float z)
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
+// 0.5 z (1 + tanh(u)) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3): 2 u
+__device__ __forceinline__ float epi_tanh_arg(float z) { return 1.59576912160573071176f * __builtin_fmaf(0.044715f * z * z, z, z); }
+
 __device__ __forceinline__ float epi_act(float z, int act)
 {
     switch (act) {
         case DMM_ACT_RELU: return z < 0.f ? 0.f : z;   // keeps NaN
         case DMM_ACT_SILU: return z * epi_sigmoid(z);
         case DMM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
-        // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3)
-        case DMM_ACT_GELU_TANH: return z * epi_sigmoid(1.59576912160573071176f * __builtin_fmaf(0.044715f * z * z, z, z));
+        case DMM_ACT_GELU_TANH: return z * epi_sigmoid(epi_tanh_arg(z));
         default: return z;
     }
 }
@@ -87,14 +89,24 @@ __device__ __forceinline__ void epi_store1(const Epi &e, const EpiScale &sc, flo
     else reinterpret_cast<half_t *>(e.y)[i] = (half_t)z;
 }
 
-// The activation of four values.  kSmall: one after the other in a loop (the vector turned by one element each
-// time), a quarter of the code and of the registers, for kernels that have none to spare; else side by side, which
-// hides the latency where few waves run.
+// The activation of four values side by side, which hides the latency of the exponentials.  kSmall: erf, by far the
+// longest, one value after the other in a loop (the vector turned by one element each time), for kernels that
+// have no registers to spare.
 template <bool kSmall>
 __device__ __forceinline__ f4_t epi_act4(f4_t z, int act)
 {
+    if (act == DMM_ACT_NONE) return z;
+    if (act == DMM_ACT_SILU || act == DMM_ACT_GELU_TANH) {
+        f4_t t = z;
+        if (act == DMM_ACT_GELU_TANH) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] = epi_tanh_arg(z[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) z[i] *= epi_sigmoid(t[i]);
+        return z;
+    }
     if constexpr (kSmall) {
-        if (act == DMM_ACT_NONE) return z;
 #pragma unroll 1
         for (int i = 0; i < 4; i++) z = f4_t{z[1], z[2], z[3], epi_act(z[0], act)};
     } else {
