@@ -31,6 +31,7 @@ namespace dmm {
 #include "dmm_gemm.h"
 #include "dmm_epilogue.h"
 #include "dmm_ops_rows.h"
+#include "dmm_ops_mid.h"
 #include "dmm_ops_gemm.h"
 #include "dmm_route.h"
 #include "dmm_ops_host.h"
@@ -56,7 +57,7 @@ int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, 
 
 int dmm_set_ops_kernel(int kernel)
 {
-    if (kernel < -1 || kernel > kOpsRows8) return DMM_ERR_BAD_SHAPE;
+    if (kernel < -1 || kernel > kOpsMid) return DMM_ERR_BAD_SHAPE;
     return g_ops_kernel.exchange(kernel, std::memory_order_relaxed);
 }
 

@@ -82,7 +82,7 @@ int run_ops_gemm(const void *x, const void *codes, const void *grid, const Group
 
 // dmm_set_ops_kernel: what a test or a benchmark forces instead of the choice below (-1: nothing)
 std::atomic<int> g_ops_kernel{-1};
-enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3, kOpsRows8 = 4 };
+enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3, kOpsRows8 = 4, kOpsMid = 5 };
 
 template <int NT, int XI, int W, int CG, bool kGated, bool kOne>
 int launch_ops_rows_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
@@ -148,6 +148,16 @@ int launch_ops_stream(const void *x, const void *codes, const void *grid, const 
     return launch(ops_stream_kernel, dim3((unsigned)tiles), dim3(1024), (size_t)ops_stream_lds(K), s, args);
 }
 
+// tens of rows per expert, 32 per segment
+template <bool kGated>
+int launch_ops_mid(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
+{
+    const int64_t units = ops_segments(g, kMidRows) * ((e.N + 15) / 16);
+    const int64_t wgs = units < cu_count() ? units : cu_count();
+    const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, 0, 0};
+    return launch(ops_mid_kernel<4, kGated>, dim3((unsigned)wgs), dim3(64 * kMidW), (size_t)kMidBytes, s, args);
+}
+
 template <int NT, int D, bool kGated>
 int launch_ops_q8d_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
                         hipStream_t s)
@@ -209,6 +219,7 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     if (rows8_ok && (force == kOpsRows8 || (force < 0 && g.R <= 2 && gemv_q8_enabled())))
         return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && (force == kOpsRows || (force < 0 && g.R / g.E <= 32))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    if (rows_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
     if (force != kOpsGemm && !g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 &&
         gemm_reg_ok(g.R, rows, K)) {
         const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cu_count());
@@ -270,6 +281,7 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_ROUTE(1, 64), DMM_K_ROUTE(2, 64), DMM_K_ROUTE(4, 64), DMM_K_ROUTE(8, 64), DMM_K_ROUTE(16, 64),
 #undef DMM_K_ROUTE
         kinfo(route_place_kernel, kLdsMax, false), kinfo(ops_stream_kernel, kLdsMax, true),
+        kinfo(ops_mid_kernel<4, false>, kMidBytes, true), kinfo(ops_mid_kernel<4, true>, kMidBytes, true),
     };
     return t;
 }

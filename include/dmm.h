@@ -329,7 +329,8 @@ int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const 
 
 /* Forces a kernel of the two products where the library would choose, process-wide, for tests and measurement:
  * 0 the catch-all, 1 the kernel for few rows, 2 the matrix-matrix kernel, 3 the same with split K (where a
- * workspace is given); -1: the library's own choice.  A forced kernel that cannot take a call leaves it to one that
+ * workspace is given), 4 the kernel for few rows on 8-bit operands (half outputs), 5 the kernel for tens of rows;
+ * -1: the library's own choice.  A forced kernel that cannot take a call leaves it to one that
  * can.  Returns the previous value (>= -1), or DMM_ERR_BAD_SHAPE.  Results differ by the order of the sums only. */
 int dmm_set_ops_kernel(int kernel);
 

@@ -26,7 +26,7 @@ def sixteen_bit_operands():
     capi.lib().dmm_set_gemv_8bit(before)
 
 
-@pytest.fixture(params=[-1, 1, 2, 3, 4], ids=["auto", "rows", "gemm", "split", "rows8"])
+@pytest.fixture(params=[-1, 1, 2, 3, 4, 5], ids=["auto", "rows", "gemm", "split", "rows8", "mid"])
 def kernel(request):
     """The library's choice, and every kernel in its place where it can take the call."""
     lib = capi.lib()
