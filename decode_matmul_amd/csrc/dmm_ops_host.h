@@ -215,7 +215,7 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
         return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
     // 8-bit operands: a job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored
     // twice, which a residual that is the output itself would not survive
-    const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 31LL * 16 * 2 * cu_count());
+    const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cu_count());
     if (rows8_ok && (force == kOpsRows8 || (force < 0 && g.R <= 2 && gemv_q8_enabled())))
         return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && (force == kOpsRows || (force < 0 && g.R / g.E <= 32))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);

@@ -46,31 +46,22 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
 
     const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
     OpsCursor cur{};
-    if (!ops_range<kMidRows, NU>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
-    cur = OpsCursor{uniform(cur.expert), uniform(cur.row), uniform(cur.row_end), uniform(cur.unit), uniform(cur.left), 0};
-
+    if (!ops_range<kMidRows, NU, NU / 4>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
     struct Job {
-        int expert, row, row_end, unit, n;   // n == 0: none
+        OpsItem it;
+        int row[4];   // byte offsets of this wave's rows of x, 8 i + wave; kOut: none
     };
-    // full jobs first, what is left of the segment last: the busiest wave has the fewest tiles that way
     auto next_job = [&]() {
-        Job j{cur.expert, cur.row, cur.row_end, cur.unit, 0};
-        if (cur.left == 0) return j;
-        const int in_seg = cur.left < upn - cur.unit ? cur.left : upn - cur.unit;
-        j.n = in_seg < NU ? in_seg : NU;
-        j.row_end = cur.row + kMidRows < cur.row_end ? cur.row + kMidRows : cur.row_end;
-        cur.left -= j.n;
-        cur.unit += j.n;
-        if (cur.unit == upn && cur.left > 0) {   // on to the next segment
-            cur.unit = 0;
-            cur.row += kMidRows;
-            if (cur.row >= cur.row_end && g.offsets) {
-                GroupRange r{0, 0};
-                while (r.lo == r.hi && cur.expert + 1 < g.E) r = uniform_range(g, ++cur.expert);
-                cur.row = r.lo;
-                cur.row_end = r.hi;
-            }
+        Job j{ops_next_job<kMidRows>(g, cur), {kOut, kOut, kOut, kOut}};
+        int t[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int m = j.it.row + 8 * i + wave, mc = m < g.R ? m : g.R - 1;
+            t[i] = g.rows ? uniform_load(g.rows, mc) : m;
         }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (j.it.n > 0 && j.it.row + 8 * i + wave < j.it.row_end && (uint32_t)t[i] < (uint32_t)g.T) j.row[i] = t[i] * K * 2;
         return j;
     };
 
@@ -82,13 +73,8 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
         const int xoff = chunk * kMidChunk + lane * 8 < K ? lane * 16 : kOut;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const int m = j.row + 8 * i + wave;
-            int base = kOut;
-            if (j.n > 0 && m < j.row_end) {
-                const int t = g.rows ? uniform_load(g.rows, m) : m;
-                if (t >= 0 && t < g.T) base = t * K * 2 + chunk * (kMidChunk * 2);
-            }
-            xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, base != kOut ? xoff : kOut, base != kOut ? base : 0, 0);
+            const bool ok = j.row[i] != kOut;
+            xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, ok ? xoff : kOut, ok ? j.row[i] + chunk * (kMidChunk * 2) : 0, 0);
         }
     };
     const uint32_t xs = lds_addr(smem_raw) + (uint32_t)kSTablesBytes;
@@ -105,10 +91,10 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
     // the code word of tile t for a step (of the job's K); nothing where the tile or the step does not exist
     auto issue = [&](const Job &j, int step, int t) {
         const int u = wave + (kGated ? t >> 1 : t) * W;
-        const bool ok = u < j.n && step < n_steps;
+        const bool ok = u < j.it.n && step < n_steps;
         const __amdgpu_buffer_rsrc_t crsrc = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t *>(codes) + (int64_t)j.expert * w_rows * (K >> 3), 0, w_rows * row_bytes, 0x00020000);
-        const int wrow = (j.unit + u) * 16 + (kGated ? (t & 1) * N : 0);
+            const_cast<uint16_t *>(codes) + (int64_t)j.it.expert * w_rows * (K >> 3), 0, w_rows * row_bytes, 0x00020000);
+        const int wrow = (j.it.unit + u) * 16 + (kGated ? (t & 1) * N : 0);
         cw[t] = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? wrow * row_bytes + step * 64 : kOut, 0);
     };
 
@@ -129,8 +115,8 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
         for (int gi = 0; gi < CG; gi++) acc[t][gi] = f4_t{0.f, 0.f, 0.f, 0.f};
 
     int buf = 0;
-    while (job.n > 0) {
-        const int mine = (job.n - wave + W - 1) / W * (kGated ? 2 : 1);   // this wave's tiles (0 or fewer: none)
+    while (job.it.n > 0) {
+        const int mine = (job.it.n - wave + W - 1) / W * (kGated ? 2 : 1);   // this wave's tiles (0 or fewer: none)
         Job nx = job;
         for (int c = 0; c < n_chunks; c++) {
             const bool last = c + 1 == n_chunks;
@@ -158,15 +144,15 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
         // D layout of 16x16: lane holds rows 4 q + i of W against column c16, i.e. outputs n = 16 unit + 4 q + i of row c16
         if (mine > 0) {
             const Epi epi = rows_args_copy().epi;
-            const EpiScale sc = epi_scale(epi, job.expert);
+            const EpiScale sc = epi_scale(epi, job.it.expert);
 #pragma unroll
             for (int t = 0; t < NT; t += kGated ? 2 : 1) {
                 if (t >= mine) break;
-                const int n = (job.unit + wave + (kGated ? t >> 1 : t) * W) * 16 + 4 * q;
+                const int n = (job.it.unit + wave + (kGated ? t >> 1 : t) * W) * 16 + 4 * q;
 #pragma unroll
                 for (int gi = 0; gi < CG; gi++) {
-                    const int m = job.row + gi * 16 + c16;
-                    if (m < job.row_end) epi_store4<kGated, true>(epi, sc, acc[t][gi], acc[kGated ? t + 1 : t][gi], m, n, job.expert);
+                    const int m = job.it.row + gi * 16 + c16;
+                    if (m < job.it.row_end) epi_store4<kGated, true>(epi, sc, acc[t][gi], acc[kGated ? t + 1 : t][gi], m, n, job.it.expert);
                 }
             }
         }

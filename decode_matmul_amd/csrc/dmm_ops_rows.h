@@ -3,11 +3,12 @@
 
 // ------------------------------------------------------------------ the work, cut into jobs
 // A segment is up to SR rows of y of one expert (a dense call is one expert); a unit is a segment times 16 columns of
-// y: one 16-row tile of W, or for a gated call two, the gate's and the up projection's.  All units are numbered,
-// segment by segment, and dealt out as contiguous ranges that differ by at most one unit, one range per
-// workgroup and one workgroup per compute unit, whatever the experts' sizes are: an expert with many rows simply has more
-// segments, and the workgroups that walk its other segments at the same time find its codes in the caches.  A
-// workgroup goes through its range in jobs of up to NU units of one segment.
+// y: one 16-row tile of W, or for a gated call two, the gate's and the up projection's.  Every segment is cut into the same
+// number of jobs, whose sizes differ by at most one unit, and the jobs of all segments are dealt out as contiguous ranges
+// that differ by at most one job, one range per workgroup and one workgroup per compute unit, whatever the experts'
+// sizes are: an expert with many rows simply has more segments, and the workgroups that walk its other segments at the
+// same time find its codes in the caches.  The number of jobs per segment is the one that a cost of kFixed units per job
+// and one per unit favours: as many as r rounds of jobs have room for, for the best of four r.
 //
 // A job is what gemv_f16d_kernel does: chunk of k steps outside, one step per wave; the slice of x of the step
 // through the wave's own piece of LDS into eight B operands; tiles inside, every tile's accumulator in registers; code
@@ -17,8 +18,8 @@
 // LDS map: tables [0, 96K), then W pieces of XI KB.
 struct OpsCursor {
     int expert, row, row_end;   // segment: rows row .. of an expert whose rows end at row_end
-    int unit, left;             // next unit inside the segment, units left in the range
-    int per;                    // units per job in this segment
+    int part, left;             // next job inside the segment, jobs left in the range
+    int parts, base, extra;     // jobs per segment; units per job, one more for the first `extra` of them
 };
 
 typedef __attribute__((address_space(4))) const int32_t const_i32_t;
@@ -52,16 +53,8 @@ __device__ __forceinline__ int wave_scan(int v, int lane)
 
 __device__ __forceinline__ int cut_up(const GroupRange &r, int by) { return (int)(((uint32_t)(r.hi - r.lo) + (uint32_t)by - 1u) / (uint32_t)by); }
 
-// the units per job for `n` units of a segment: as few jobs as possible, of even size
-template <int NU>
-__device__ __forceinline__ int per_job(int n)
-{
-    const int jobs = (n + NU - 1) / NU;
-    return jobs <= 1 ? n : (n + jobs - 1) / jobs;
-}
-
-// the workgroup's range of units; false: it has none
-template <int SR, int NU>
+// the workgroup's range of jobs; false: it has none
+template <int SR, int NU, int kFixed>
 __device__ __forceinline__ bool ops_range(const Groups &g, int upn, int lane, OpsCursor &c)
 {
     int segs, first_scan = 0;
@@ -78,12 +71,38 @@ __device__ __forceinline__ bool ops_range(const Groups &g, int upn, int lane, Op
             segs += __builtin_amdgcn_readlane(wave_scan(cut_up(r, SR), lane), 63);
         }
     }
-    const uint32_t units = (uint32_t)segs * (uint32_t)upn;   // below 2^31 (the host's business)
-    const uint32_t u0 = (uint32_t)((uint64_t)units * blockIdx.x / gridDim.x), u1 = (uint32_t)((uint64_t)units * (blockIdx.x + 1) / gridDim.x);
-    if (u0 >= u1) return false;
-    const int seg = (int)(u0 / (uint32_t)upn);
-    c.unit = (int)(u0 - (uint32_t)seg * (uint32_t)upn);
-    c.left = (int)(u1 - u0);
+    if (segs == 0) return false;
+    const uint32_t wgs = gridDim.x, least = ((uint32_t)upn + NU - 1u) / NU;   // fewest jobs a segment can be cut into
+    uint32_t parts = least;
+    {
+        // (the quotients by reciprocals: one too few or too many costs balance, nothing else)
+        const float inv = __builtin_amdgcn_rcpf((float)segs) * (float)wgs;
+        uint32_t r = (uint32_t)((float)least * __builtin_amdgcn_rcpf(inv) + 0.999f);
+        r = r < 1u ? 1u : r;
+        float best = 3e38f;
+#pragma unroll
+        for (int i = 0; i < 4; i++, r++) {
+            uint32_t p = (uint32_t)((float)r * inv + 0.001f);
+            p = p > (uint32_t)upn ? (uint32_t)upn : p < least ? least : p;
+            const float rounds = (float)(uint32_t)((float)p * __builtin_amdgcn_rcpf(inv) + 0.999f);
+            const float cost = rounds * ((float)kFixed + (float)(uint32_t)((float)upn * __builtin_amdgcn_rcpf((float)p) + 0.999f));
+            if (cost < best * 0.999f) {
+                best = cost;
+                parts = p;
+            }
+        }
+    }
+    parts = (uint32_t)uniform((int)parts);
+    const uint32_t jobs = (uint32_t)segs * parts;   // below 2^31 (the host's business)
+    const uint32_t b = blockIdx.x, q = jobs / wgs, rest = jobs - q * wgs;
+    const uint32_t j0 = b * q + (b < rest ? b : rest);
+    c.left = (int)(q + (b < rest ? 1u : 0u));
+    if (c.left == 0) return false;
+    const int seg = (int)(j0 / parts);
+    c.part = (int)(j0 - (uint32_t)seg * parts);
+    c.parts = (int)parts;
+    c.base = (int)((uint32_t)upn / parts);
+    c.extra = upn - c.base * (int)parts;
     if (!g.offsets) {
         c.expert = 0;
         c.row = seg * SR;
@@ -110,15 +129,38 @@ __device__ __forceinline__ bool ops_range(const Groups &g, int upn, int lane, Op
             base += __builtin_amdgcn_readlane(s, 63);
         }
     }
-    const int in_seg = c.left < upn - c.unit ? c.left : upn - c.unit;
-    c.per = per_job<NU>(in_seg);
+    c = OpsCursor{uniform(c.expert), uniform(c.row), uniform(c.row_end), uniform(c.part), uniform(c.left), uniform(c.parts),
+                  uniform(c.base), uniform(c.extra)};
     return true;
 }
 
-// a job's share of a chunk; n == 0: nothing
+// a job, and (few-rows kernel) its share of a chunk; n == 0: nothing
 struct OpsItem {
     int expert, row, row_end, unit, n, chunk;
 };
+
+// the next job of the range
+template <int SR>
+__device__ __forceinline__ OpsItem ops_next_job(const Groups &g, OpsCursor &c)
+{
+    OpsItem it{c.expert, c.row, c.row_end, 0, 0, 0};
+    if (c.left == 0) return it;
+    it.n = c.base + (c.part < c.extra ? 1 : 0);
+    it.unit = c.part * c.base + (c.part < c.extra ? c.part : c.extra);
+    it.row_end = c.row + SR < c.row_end ? c.row + SR : c.row_end;
+    c.left--;
+    if (++c.part == c.parts && c.left > 0) {   // on to the next segment
+        c.part = 0;
+        c.row += SR;
+        if (c.row >= c.row_end && g.offsets) {
+            GroupRange r{0, 0};
+            while (r.lo == r.hi && c.expert + 1 < g.E) r = uniform_range(g, ++c.expert);
+            c.row = r.lo;
+            c.row_end = r.hi;
+        }
+    }
+    return it;
+}
 
 // The kernel's one argument, so that its address in the constant kernel-argument segment is known.  What is needed
 // once per job (the epilogue) is read from there when it is needed, not held in scalar registers through the loop.
@@ -204,77 +246,53 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
 
     const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
     OpsCursor cur{};
+    OpsItem it;
     if constexpr (kOne) {
         const int b = (int)blockIdx.x;
-        cur.unit = b * args.units_q + (b < args.units_r ? b : args.units_r);
-        cur.left = args.units_q + (b < args.units_r ? 1 : 0);
-        cur.row_end = g.R;
+        it = OpsItem{0, 0, g.R, b * args.units_q + (b < args.units_r ? b : args.units_r), args.units_q + (b < args.units_r ? 1 : 0), 0};
     } else {
-        if (!ops_range<SR, NU>(g, upn, lane, cur)) return 0u;   // the whole workgroup, before any barrier
-        cur = OpsCursor{uniform(cur.expert), uniform(cur.row), uniform(cur.row_end), uniform(cur.unit), uniform(cur.left), uniform(cur.per)};
+        if (!ops_range<SR, NU, 4>(g, upn, lane, cur)) return 0u;   // the whole workgroup, before any barrier
+        it = ops_next_job<SR>(g, cur);
     }
-
-    // the next job, and the cursor behind it
-    auto next_job = [&]() {
-        OpsItem it{cur.expert, cur.row, cur.row_end, cur.unit, 0, 0};
-        if (cur.left == 0) return it;
-        const int in_seg = cur.left < upn - cur.unit ? cur.left : upn - cur.unit;
-        it.n = cur.per < in_seg ? cur.per : in_seg;
-        it.row_end = cur.row + SR < cur.row_end ? cur.row + SR : cur.row_end;
-        cur.left -= it.n;
-        cur.unit += it.n;
-        if (cur.unit == upn && cur.left > 0) {   // on to the next segment
-            cur.unit = 0;
-            cur.row += SR;
-            if (cur.row >= cur.row_end && g.offsets) {
-                GroupRange r{0, 0};
-                while (r.lo == r.hi && cur.expert + 1 < g.E) r = uniform_range(g, ++cur.expert);
-                cur.row = r.lo;
-                cur.row_end = r.hi;
-            }
-            cur.per = per_job<NU>(cur.left < upn ? cur.left : upn);
-        }
-        return it;
+    // Rows of x: lane l (and l + 32) of row_list holds the list's entry for row l of a job's segment.  The entries are asked
+    // for a whole job ahead, so that nobody waits for them behind the codes.
+    auto row_list = [&](const OpsItem &j) {
+        int m = j.row + (lane & 31);
+        if (g.rows) m = g.rows[m < g.R ? m : g.R - 1];
+        return m;
     };
-    auto next_item = [&](const OpsItem &it) {
-        OpsItem o = it;
-        if constexpr (kOne) {
-            o.chunk++;
-            return o;
-        }
-        if (it.n > 0 && it.chunk + 1 < n_chunks) o.chunk++;
-        else o = next_job();
-        return o;
-    };
+    OpsItem nj{};       // the job after this one
+    int r_it = 0, r_nj = 0;
+    if constexpr (!kOne) {
+        r_it = row_list(it);
+        nj = ops_next_job<SR>(g, cur);
+        r_nj = row_list(nj);
+    }
 
     const __amdgpu_buffer_rsrc_t xrsrc =
         __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(x), 0, (int)((int64_t)g.T * K * 2), 0x00020000);
-    auto x_base = [&](int m, int end) {   // byte offset of the row of x behind row m of y (uniform)
-        if (m >= end) return kOut;
-        const int t = g.rows ? uniform_load(g.rows, m) : m;
-        return t >= 0 && t < g.T ? t * K * 2 : kOut;
-    };
     u4_t xv[CG][XI];
     // load i of a slice is piece lane % 32 (16 bytes) of row 2 i + lane / 32; rows that do not exist and pieces past K
     // are zeros without a memory access
-    auto load_x = [&](const OpsItem &it, int gi) {
+    auto load_x = [&](const OpsItem &it, int rl, int gi) {
         const int step = it.chunk * W + wave;
         const bool ok = it.n > 0 && step < n_steps;
         const int piece = (int)threadIdx.x & 31;
-        const bool inside = step * 256 + piece * 8 < K;
+        const bool inside = ok && step * 256 + piece * 8 < K;
         if constexpr (kOne) {   // rows past the last lie past the end of the buffer
             const int b = inside ? ((((int)threadIdx.x >> 5) & 1) * K + piece * 8) * 2 : kOut;
 #pragma unroll
             for (int i = 0; i < XI; i++)
                 xv[gi][i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, b, ok ? step * 512 + (gi * CM + 2 * i) * 2 * K : kOut, 0);
-            return;
-        }
+        } else {
+            // byte offset of the lane's row, beyond the buffer where there is none
+            const int off = it.row + (lane & 31) < it.row_end && (uint32_t)rl < (uint32_t)g.T ? rl * K * 2 : kOut;
 #pragma unroll
-        for (int i = 0; i < XI; i++) {
-            const int m = it.row + gi * CM + 2 * i;
-            const int b0 = ok ? x_base(m, it.row_end) : kOut, b1 = ok ? x_base(m + 1, it.row_end) : kOut;
-            const int b = ((int)threadIdx.x & 32) ? b1 : b0;
-            xv[gi][i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, inside && b != kOut ? b + piece * 16 : kOut, ok ? step * 512 : 0, 0);
+            for (int i = 0; i < XI; i++) {
+                const int b0 = __builtin_amdgcn_readlane(off, gi * CM + 2 * i), b1 = __builtin_amdgcn_readlane(off, gi * CM + 2 * i + 1);
+                const int b = ((int)threadIdx.x & 32) ? b1 : b0;
+                xv[gi][i] = __builtin_amdgcn_raw_buffer_load_b128(xrsrc, inside && b != kOut ? b + piece * 16 : kOut, ok ? step * 512 : 0, 0);
+            }
         }
     };
     // the wave's piece, addressed as in gemv_f16d_kernel
@@ -293,11 +311,8 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
         cwd = __builtin_amdgcn_raw_buffer_load_b128(crsrc, voff, ok ? wrow * row_bytes + step * 64 : kOut, 0);
     };
 
-    OpsItem it;
-    if constexpr (kOne) it = OpsItem{0, 0, g.R, cur.unit, cur.left, 0};
-    else it = next_job();
 #pragma unroll
-    for (int gi = 0; gi < CG; gi++) load_x(it, gi);
+    for (int gi = 0; gi < CG; gi++) load_x(it, r_it, gi);
     u4_t cw[D];
     issue(cw[0], it, 0);   // the rest of the ring after the prologue's work, as in gemv_f16d_kernel
     uint32_t *flags = reinterpret_cast<uint32_t *>(smem_raw + kO8Flags);   // kQ8 only
@@ -367,7 +382,14 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
     while (kOne ? it.chunk < n_chunks : it.n > 0) {
         // (a value of its own every time round: what depends on it is not kept in scalar registers through the loop)
         asm volatile("" : "+s"(it.n), "+s"(it.unit));
-        const OpsItem nx = next_item(it);
+        const bool last = it.chunk + 1 == n_chunks;
+        OpsItem nx = it;
+        nx.chunk++;
+        int r_nx = r_it;
+        if (!kOne && last) {
+            nx = nj;
+            r_nx = r_nj;
+        }
         const bool step_ok = it.chunk * W + wave < n_steps;
         const int nt = kGated ? 2 * it.n : it.n;
         u4_t xb[CG][kQ8 ? 1 : 8];
@@ -378,7 +400,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
             xm = __builtin_bit_cast(h8_t, lds_read16(o8_m));
             xb0 = i8_t{(int)r0[0], (int)r0[1], (int)r0[2], (int)r0[3], (int)r1[0], (int)r1[1], (int)r1[2], (int)r1[3]};
             xb1 = i8_t{(int)r2[0], (int)r2[1], (int)r2[2], (int)r2[3], (int)r3[0], (int)r3[1], (int)r3[2], (int)r3[3]};
-            load_x(nx, 0);
+            load_x(nx, r_nx, 0);
         } else {
 #pragma unroll
             for (int gi = 0; gi < CG; gi++) {
@@ -386,7 +408,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
                 for (int i = 0; i < XI; i++) lds_write16((xs_w() ^ (uint32_t)(32 * i)) + (uint32_t)(1024 * i), xv[gi][i]);
 #pragma unroll
                 for (int i = 0; i < 8; i++) xb[gi][i] = lds_read16(xs_r ^ (uint32_t)(16 * i));
-                load_x(nx, gi);
+                load_x(nx, r_nx, gi);
             }
         }
 #pragma unroll
@@ -398,7 +420,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
             if (t + D < NT) issue(cw[t % D], it, t + D);
             else issue(cw[t % D], nx, t + D - NT);
         }
-        if (it.chunk + 1 == n_chunks) {
+        if (last) {
             // the end of a job: cell (tile, quarter, column) of every wave's piece, a group of rows at a time
             Epi epi = args.epi;
             if constexpr (!kOne) epi = rows_args_copy().epi;
@@ -493,6 +515,11 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
         }
         if constexpr (kQ8) {
             if (!kOne || nx.chunk < n_chunks) split_x();
+        }
+        if (!kOne && last) {
+            r_it = r_nj;
+            nj = ops_next_job<SR>(g, cur);
+            r_nj = row_list(nj);
         }
         it = nx;
     }
