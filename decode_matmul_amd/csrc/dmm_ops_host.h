@@ -189,15 +189,35 @@ int launch_ops_q8d(const void *x, const void *codes, const void *grid, const Gro
     }
 }
 
-// rows of a segment by the rows an expert has
+// Rows of a segment, and waves.  Dense: as many rows as there are.  By expert, where only the average is known: sixteen rows on
+// eight waves, except for less than one row per expert on a long K (graph launches, us, four rows on sixteen waves / sixteen
+// on eight: 2 x 11008 x 4096, 8 experts, 4 rows 20.6 / 21.6, 8 rows 32.9 / 33.3, 32 rows 81.7 / 58.0; 4096 x 11008, 16 experts, 4 rows
+// 13.0 / 16.2, 16 rows 32.7 / 27.8; 2 x 1408 x 2048, 64 experts, 16 rows 17.1 / 15.3, 256 rows 58.4 / 33.4; eight rows on sixteen
+// waves are behind one or the other).  Up to 2048 k there are no more than eight steps: half of sixteen waves would have none.
+// 32 rows per segment where an expert has more than sixteen.
 template <bool kGated>
 int run_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
 {
-    const int64_t rows = g.offsets ? std::min<int64_t>(g.R, 2 * (int64_t)g.R / g.E + 2) : g.R;
-    if (rows <= 4) return launch_ops_rows<2, 16, 1, kGated>(x, codes, grid, g, e, K, s);
-    if (rows <= 8) return launch_ops_rows<4, 16, 1, kGated>(x, codes, grid, g, e, K, s);
-    if (rows <= 16) return launch_ops_rows<8, 8, 1, kGated>(x, codes, grid, g, e, K, s);
-    return launch_ops_rows<8, 8, 2, kGated>(x, codes, grid, g, e, K, s);
+    const bool short_k = K <= 2048;
+    if (g.offsets ? g.R > 16 * (int64_t)g.E : g.R > 16) return launch_ops_rows<8, 8, 2, kGated>(x, codes, grid, g, e, K, s);
+    if (!short_k && (g.R <= 4 || (g.offsets && g.R < g.E && K >= 4096))) return launch_ops_rows<2, 16, 1, kGated>(x, codes, grid, g, e, K, s);
+    if (!short_k && !g.offsets && g.R <= 8) return launch_ops_rows<4, 16, 1, kGated>(x, codes, grid, g, e, K, s);
+    return launch_ops_rows<8, 8, 1, kGated>(x, codes, grid, g, e, K, s);
+}
+
+// More than 32 rows, dense: the few-rows kernel (32 rows per segment) or split K / the matrix-matrix kernel.  The first costs
+// about 7 us, K * 0.34 ns per 16-row tile of the busiest workgroup and 3.5 us for every eight of them after the first;
+// the split what passes_beat_splitk says, 14 us + 0.085 per row + 0.3 per MB of codes (graph launches, us, few rows / split:
+// 4096 x 4096 M = 64 11.6 / 20.8, 256 20.0 / 27.0, 400 33.6 / 31.2; 8192 x 8192 M = 128 31.2 / 32.4, 200 54.4 / 42.6; 4096 x 11008 M = 128
+// 26.4 / 29.8; 2 x 11008 x 4096 M = 64 30.2 / 26.2).
+bool ops_rows_beat_split(int64_t M, int64_t N, int64_t K, bool gated, int cus)
+{
+    if (M <= 32) return true;
+    if (M > 512) return false;
+    const int64_t units = (M + 31) / 32 * ((N + 15) / 16), tiles = (units + cus - 1) / cus * (gated ? 2 : 1);
+    const double rows = 7.0 + (double)tiles * (double)K * 0.34e-3 + 3.5 * (double)((tiles - 1) / 8);
+    const double split = 14.0 + 0.085 * (double)M + 0.3e-6 * (double)(gated ? 2 * N : N) * (double)(K >> 2) * (256.0 / cus);
+    return rows * 1.05 < split;
 }
 
 template <bool kGated>
@@ -208,21 +228,38 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
     if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
     const bool rows_ok = ops_segments(g, 2) * ((e.N + 15) / 16) < (1LL << 31);
-    if (!kGated && force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0 && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cu_count() &&
-        ops_stream_lds(K) <= kLdsMax)
+    const int cus = cu_count();
+    // One row of a matrix: the batch-1 kernels' bodies
+    const bool one_row = force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0;
+    if (!kGated && one_row && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cus && ops_stream_lds(K) <= kLdsMax)
         return launch_ops_stream(x, codes, grid, g, e, K, s);
-    if (force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0 && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled())
-        return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
-    // 8-bit operands: a job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored
-    // twice, which a residual that is the output itself would not survive
-    const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cu_count());
-    if (rows8_ok && (force == kOpsRows8 || (force < 0 && g.R <= 2 && gemv_q8_enabled())))
+    if (one_row && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled()) return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
+    // 8-bit operands, two rows per segment: one or two rows of a dense call, and by expert where few experts have a row and
+    // the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7 us, 16-bit 14.4; 2 rows 18.9 / 21.1; but 4 rows 24.7 / 20.6).  A
+    // job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored twice,
+    // which a residual that is the output itself would not survive.
+    const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cus);
+    const bool rows8_pays = g.offsets ? (g.R <= 2 || 4 * (int64_t)g.R <= g.E) && K >= 4096 &&
+                                            std::min<int64_t>(g.R, g.E) * rows * (K >> 2) >= (20LL << 20)
+                                      : g.R <= 2;
+    if (rows8_ok && (force == kOpsRows8 || (force < 0 && rows8_pays && gemv_q8_enabled())))
         return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
-    if (rows_ok && (force == kOpsRows || (force < 0 && g.R / g.E <= 32))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    if (rows_ok && force == kOpsRows) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
-    if (force != kOpsGemm && !g.offsets && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 &&
-        gemm_reg_ok(g.R, rows, K)) {
-        const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cu_count());
+    if (g.offsets) {
+        // Up to eight rows per expert the few-rows kernel, up to 160 the one for tens of rows where every wave has a unit
+        // (graph launches, us, few rows / tens / matrix-matrix, rows per expert: 2 x 11008 x 4096, 8 experts 6: 58 / 66 / 88, 12: 77 / 68 /
+        // 90, 31: 126 / 98 / 180, 64: 222 / 165 / 218, 128: - / 288 / 361, 256: - / 529 / 534; 4096 x 11008, 16 experts 8: 73 / 75 / 141, 31: 113 / 98 /
+        // 147, 128: - / 287 / 291, 256: - / 541 / 451; 2 x 1408 x 2048, 64 experts 8: 44 / 47 / 66, 31: 94 / 68 / 98, 128: - / 163 / 196, 256: - /
+        // 299 / 273; but 4096 x 4096, 8 experts, 8 units per workgroup, 12: 20 / 24)
+        const int64_t avg = g.R / g.E, units = (int64_t)g.E * ((avg + 31) / 32) * ((e.N + 15) / 16);
+        if (force < 0 && rows_ok && (avg < 8 || (avg <= 64 && units <= 8LL * cus))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+        if (force < 0 && rows_ok && avg < 160) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
+        return run_ops_gemm<kGated>(x, codes, grid, g, e, K, s);
+    }
+    if (force < 0 && rows_ok && ops_rows_beat_split(g.R, e.N, K, kGated, cus)) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    if (force != kOpsGemm && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 && gemm_reg_ok(g.R, rows, K)) {
+        const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cus);
         if (splits >= 2) {
             const int st = launch_gemm_partial(x, codes, grid, (float *)workspace, splits, g.R, rows, K, s);
             if (st != 0) return st;
@@ -246,6 +283,7 @@ int64_t ops_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated)
 {
     const int64_t rows = gated ? 2 * N : N;
     if (M < kSplitKMinM || N < 1 || K < 64 || (K & 63) || M > 65535LL * 128 || !gemm_reg_ok(M, rows, K)) return 0;
+    if (ops_rows_beat_split(M, N, K, gated, cu_count_or_default()) && g_ops_kernel.load(std::memory_order_relaxed) != kOpsSplit) return 0;
     const int splits = splitk_plan(M, rows, K, INT64_MAX, cu_count_or_default());
     return splits >= 2 ? (int64_t)splits * M * rows * 4 : 0;
 }
