@@ -46,7 +46,10 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
 
     const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
     OpsCursor cur{};
-    if (!ops_range<kMidRows, NU, NU / 4>(g, upn, lane, cur)) return;   // the whole workgroup, before any barrier
+    const GroupRange first = ops_first_ranges(g, lane);
+    stream_stage_signs<64 * W>(smem_raw, tid);   // needs no load: while the list of the experts' rows is on its way
+    __builtin_amdgcn_sched_barrier(0);
+    if (!ops_range<kMidRows, NU, NU / 4>(g, first, upn, lane, cur)) return;   // the whole workgroup, before any barrier
     struct Job {
         OpsItem it;
         int row[4];   // byte offsets of this wave's rows of x, 8 i + wave; kOut: none
@@ -102,8 +105,6 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
     load_x(job, 0);
 #pragma unroll
     for (int t = 0; t < NT; t++) issue(job, 0, t);
-    stream_stage_signs<64 * W>(smem_raw, tid);
-    __builtin_amdgcn_sched_barrier(0);
     stream_stage_grid<64 * W>(smem_raw, grow, tid);
     store_x(0);
     __syncthreads();

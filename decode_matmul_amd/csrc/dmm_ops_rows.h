@@ -53,16 +53,22 @@ __device__ __forceinline__ int wave_scan(int v, int lane)
 
 __device__ __forceinline__ int cut_up(const GroupRange &r, int by) { return (int)(((uint32_t)(r.hi - r.lo) + (uint32_t)by - 1u) / (uint32_t)by); }
 
+// the first 64 experts' rows, one per lane: asked for at a kernel's start, ahead of work that needs no list
+__device__ __forceinline__ GroupRange ops_first_ranges(const Groups &g, int lane)
+{
+    GroupRange first{0, 0};
+    if (g.offsets && lane < g.E) first = group_range(g, lane);
+    return first;
+}
+
 // the workgroup's range of jobs; false: it has none
 template <int SR, int NU, int kFixed>
-__device__ __forceinline__ bool ops_range(const Groups &g, int upn, int lane, OpsCursor &c)
+__device__ __forceinline__ bool ops_range(const Groups &g, const GroupRange &first, int upn, int lane, OpsCursor &c)
 {
     int segs, first_scan = 0;
-    GroupRange first{0, 0};
     if (!g.offsets) {
         segs = (g.R + SR - 1) / SR;
     } else {
-        if (lane < g.E) first = group_range(g, lane);
         first_scan = wave_scan(cut_up(first, SR), lane);
         segs = __builtin_amdgcn_readlane(first_scan, 63);
         for (int e0 = 64; e0 < g.E; e0 += 64) {
@@ -245,13 +251,30 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
     constexpr int kOut = (int)0x80000000;
 
     const u4_t grow = tid < 256 ? reinterpret_cast<const u4_t *>(args.grid)[tid] : u4_t{0u, 0u, 0u, 0u};
+    // the sign rows need no load: written while the list of the experts' rows is on its way
+    auto stage_signs = [&]() {
+        if constexpr (kQ8) {
+            if (tid >= 256 && tid < 512) {
+                const int t = tid - 256, row = t >> 1;
+                const u2_t sb = sign_bytes((uint32_t)row);
+                const uint32_t sg = lds_addr(smem_raw) + (uint32_t)((row * 16 + (t & 1) * 8 + (row & 7)) * 16);
+#pragma unroll
+                for (int i = 0; i < 8; i++) lds_write16(sg ^ (uint32_t)(i * 16), u4_t{sb[0], sb[1], sb[0], sb[1]});
+            }
+        } else {
+            stream_stage_signs<64 * W>(smem_raw, tid);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
     OpsCursor cur{};
     OpsItem it;
     if constexpr (kOne) {
         const int b = (int)blockIdx.x;
         it = OpsItem{0, 0, g.R, b * args.units_q + (b < args.units_r ? b : args.units_r), args.units_q + (b < args.units_r ? 1 : 0), 0};
     } else {
-        if (!ops_range<SR, NU, 4>(g, upn, lane, cur)) return 0u;   // the whole workgroup, before any barrier
+        const GroupRange first = ops_first_ranges(g, lane);
+        stage_signs();
+        if (!ops_range<SR, NU, 4>(g, first, upn, lane, cur)) return 0u;   // the whole workgroup, before any barrier
         it = ops_next_job<SR>(g, cur);
     }
     // Rows of x: lane l (and l + 32) of row_list holds the list's entry for row l of a job's segment.  The entries are asked
@@ -316,6 +339,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
     u4_t cw[D];
     issue(cw[0], it, 0);   // the rest of the ring after the prologue's work, as in gemv_f16d_kernel
     uint32_t *flags = reinterpret_cast<uint32_t *>(smem_raw + kO8Flags);   // kQ8 only
+    if constexpr (kOne) stage_signs();
     if constexpr (kQ8) {
         bool exact = true;
         if (tid < 256) {
@@ -323,22 +347,14 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
             const uint32_t gg = lds_addr(smem_raw) + (uint32_t)(kSSignBytes + (tid * 16 + (tid & 15)) * 16);   // slot i ^ (tid % 16)
 #pragma unroll
             for (int i = 0; i < 16; i++) lds_write16(gg ^ (uint32_t)(i * 16), u4_t{g8[0], g8[1], g8[0], g8[1]});
-        } else if (tid < 512) {
-            const int t = tid - 256, row = t >> 1;
-            const u2_t sb = sign_bytes((uint32_t)row);
-            const uint32_t sg = lds_addr(smem_raw) + (uint32_t)((row * 16 + (t & 1) * 8 + (row & 7)) * 16);
-#pragma unroll
-            for (int i = 0; i < 8; i++) lds_write16(sg ^ (uint32_t)(i * 16), u4_t{sb[0], sb[1], sb[0], sb[1]});
-        } else if (tid < 528) {
+        } else if (tid >= 512 && tid < 528) {
             flags[16 + tid - 512] = 0u;   // the two words, and what lies up to the zeros
-        } else if (tid < 544) {
+        } else if (tid >= 528 && tid < 544) {
             flags[32 + tid - 528] = 0u;   // the zero bytes the idle columns read
         }
         const bool bad = __builtin_amdgcn_ballot_w64(!exact) != 0;
         if (lane == 0) flags[wave] = bad ? 1u : 0u;
     } else {
-        stream_stage_signs<64 * W>(smem_raw, tid);
-        __builtin_amdgcn_sched_barrier(0);
         stream_stage_grid<64 * W>(smem_raw, grow, tid);
     }
     // kQ8: the slice of x that has arrived into terms and means, in the wave's piece: for the first item beside the other
