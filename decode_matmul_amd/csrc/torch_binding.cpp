@@ -421,6 +421,18 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
     return y;
 }
 
+// A contiguous tensor over a part of buf's memory, from byte `at` on; at moves past it, to the next multiple of 16.
+// (Five small results: one allocation and five of these cost the host a third of five allocations.)
+torch::Tensor carve(const torch::Tensor &buf, torch::ScalarType type, c10::IntArrayRef sizes, int64_t &at)
+{
+    torch::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    const int64_t item = static_cast<int64_t>(c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(at / item);
+    at = (at + t.numel() * item + 15) / 16 * 16;
+    return t;
+}
+
 std::vector<torch::Tensor> route_experts(torch::Tensor logits, int64_t k, const std::string &scoring, bool normalize)
 {
     check_device(logits.device(), "route_experts");
@@ -434,12 +446,13 @@ std::vector<torch::Tensor> route_experts(torch::Tensor logits, int64_t k, const 
     const int sc = scoring == "sigmoid" ? DMM_SCORE_SIGMOID : DMM_SCORE_SOFTMAX;
     c10::OptionalDeviceGuard guard;
     if (logits.is_cuda()) guard.reset_device(logits.device());
-    const auto i32 = logits.options().dtype(torch::kInt32).requires_grad(false);
-    torch::Tensor weights = torch::empty({T, k}, i32.dtype(torch::kFloat)), experts = torch::empty({T, k}, i32),
-                  offsets = torch::empty({E + 1}, i32), rows = torch::empty({T * k}, i32), slots = torch::empty({T, k}, i32);
-    torch::Tensor workspace;
     const int64_t ws_bytes = logits.is_cuda() ? dmm_route_workspace_bytes(T, E) : 0;
-    if (ws_bytes > 0) workspace = torch::empty({ws_bytes}, i32.dtype(torch::kUInt8));
+    torch::Tensor buf = torch::empty({16 * T * k + 4 * (E + 1) + 5 * 16 + ws_bytes}, logits.options().dtype(torch::kUInt8).requires_grad(false));
+    int64_t at = 0;
+    torch::Tensor weights = carve(buf, torch::kFloat, {T, k}, at), experts = carve(buf, torch::kInt32, {T, k}, at),
+                  offsets = carve(buf, torch::kInt32, {E + 1}, at), rows = carve(buf, torch::kInt32, {T * k}, at),
+                  slots = carve(buf, torch::kInt32, {T, k}, at);
+    void *workspace = static_cast<char *>(buf.data_ptr()) + at;   // behind the results
     hipStream_t stream = stream_of(logits.device());
     int st;
     {
@@ -448,7 +461,7 @@ std::vector<torch::Tensor> route_experts(torch::Tensor logits, int64_t k, const 
                                                       experts.data_ptr(), offsets.data_ptr(), rows.data_ptr(), slots.data_ptr())
                              : dmm_route_experts(logits.data_ptr(), type, T, E, k, sc, normalize, weights.data_ptr(), experts.data_ptr(),
                                                  offsets.data_ptr(), rows.data_ptr(), slots.data_ptr(),
-                                                 ws_bytes > 0 ? workspace.data_ptr() : nullptr, ws_bytes, stream);
+                                                 ws_bytes > 0 ? workspace : nullptr, ws_bytes, stream);
     }
     check_status(st, "route_experts");
     return {weights, experts, offsets, rows, slots};

@@ -229,6 +229,27 @@ def test_grouped_lists_that_lead_out_of_the_buffers(kernel):
             assert torch.all(out[0] == 0) and torch.all(out[-1] == 0)
 
 
+def test_grouped_rows_of_others_may_hold_anything():
+    """NaN and infinities in the rows of x of one expert and behind the last one reach no other expert's rows."""
+    for counts in ((3, 2, 5), (40, 3, 70), (300, 10, 200)):
+        for kernel in (-1, 1, 2, 4, 5):
+            capi.lib().dmm_set_ops_kernel(kernel)
+            try:
+                x, codes, grid, offsets, _, _ = grouped_inputs(counts, 0, 52, 320, False, None, False, seed=8, behind=9, coarse=True)
+                lo, hi = int(offsets[1]), int(offsets[2])
+                x[lo:hi] = math.nan
+                x[int(offsets[3]):] = math.inf
+                y = dmm.decode_matmul_grouped(*dev(x, codes, grid), 0.1, offsets.to(DEV))
+                want, tol = grouped64(x, codes, grid, 0.1, offsets, None, None, False, "none", F16, 52)
+                keep = torch.ones(x.shape[0], dtype=torch.bool)
+                keep[lo:hi] = False
+                keep[int(offsets[3]):] = False
+                assert_within(y.cpu()[keep], want[keep], tol[keep], "kernel %d" % kernel)
+                assert torch.isnan(y[lo:hi]).all()
+            finally:
+                capi.lib().dmm_set_ops_kernel(-1)
+
+
 def test_grouped_empty():
     x, codes, grid, offsets, rows, _ = grouped_inputs((0, 0), 4, 64, 256, False, None, True, seed=3)
     assert dmm.decode_matmul_grouped(*dev(x, codes, grid), 0.1, offsets.to(DEV), rows=rows.to(DEV)).shape == (0, 64)
@@ -377,6 +398,22 @@ def test_calls_on_another_stream_and_twice_at_once():
             outs.append(dmm.decode_matmul_fused(*args, 0.02, bias=bd, activation="silu", gated=True, residual=rd))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+def test_routing_results_stand_alone():
+    """The five results share one allocation and nothing else: each is contiguous, may be written, and outlives the others."""
+    logits = torch.randn(70, 12, device=DEV)
+    r = dmm.route_experts(logits, 3)
+    kept = [t.clone() for t in r]
+    for t in r:
+        assert t.is_contiguous() and not t.requires_grad and t.data_ptr() % 16 == 0
+    r.weights.zero_()
+    r.rows.fill_(-5)
+    assert torch.equal(r.experts, kept[1]) and torch.equal(r.offsets, kept[2]) and torch.equal(r.slots, kept[4])
+    slots = r.slots
+    del r
+    torch.empty(1 << 20, device=DEV).fill_(3)
+    assert torch.equal(slots, kept[4])
 
 
 def test_mixed_devices_are_refused():
