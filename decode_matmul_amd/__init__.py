@@ -152,8 +152,8 @@ def decode_matmul_grouped(x, codes, grid, scale, offsets, *, rows=None, bias=Non
     codes [E, N, K/8] (gated: [E, 2 N, K/8]), bias [E, ...] one value per row of codes, scale a number, float32 [E], or
     for a gated call float32 [E, 2]; offsets int32 [E + 1] and rows int32 [R] live on x's device and are not read by the
     host (`route_experts` makes both).  An entry of rows outside x stands for a row of zeros.  Rows from
-    offsets[E] on are not written: in `out` (optional, [R, N]) they stay as they were, in a result allocated here
-    their content is undefined."""
+    offsets[E] on are not written: in `out` (optional, [R, N], no memory shared with an input) they stay as they were, in a
+    result allocated here their content is undefined."""
     scales = scale if isinstance(scale, _torch.Tensor) else None
     return _ext().decode_matmul_grouped(x, codes, grid, 1.0 if scales is not None else float(scale), scales, offsets, rows, bias,
                                         activation, bool(gated), out_dtype or (out.dtype if out is not None else _torch.float16), out)
@@ -163,8 +163,8 @@ Routing = _collections.namedtuple("Routing", "weights experts offsets rows slots
 
 
 def route_experts(logits, k, *, scoring="softmax", normalize=True):
-    """The k largest logits of every row of logits [T, E] (half, bfloat16 or float32), equal ones by index, and the lists
-    that `decode_matmul_grouped` and `combine_experts` read.  Returns a `Routing`:
+    """The k largest logits of every row of logits [T, E] (half, bfloat16 or float32; T up to 2^24, E up to 1024, k up to
+    64), equal ones by index, and the lists that `decode_matmul_grouped` and `combine_experts` read.  Returns a `Routing`:
 
         weights  float32 [T, k]   softmax over the row, or sigmoid, of the chosen; divided by their sum if normalize
         experts  int32 [T, k]     -1: no choice (a logit of -inf or NaN is never chosen; such a weight is 0)

@@ -90,7 +90,7 @@ int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const 
 
 int64_t dmm_route_workspace_bytes(int64_t T, int64_t E)
 {
-    if (T < 1 || E < 1 || E > kRouteMaxE) return 0;
+    if (T < 1 || T > kRouteMaxT || E < 1 || E > kRouteMaxE) return 0;
     const int64_t blocks = route_blocks(T);
     return blocks == 1 ? 0 : E * (blocks * 8 * route_words(T) + (blocks + 3) / 4 * 16);
 }
@@ -202,7 +202,9 @@ int dmm_route_experts_host(const void *logits, int logits_type, int64_t T, int64
             if (best < 0) break;
             if (n == 0) big = bv;
             ex[t * k + n] = best;
-            w[t * k + n] = scoring == DMM_SCORE_SIGMOID ? 1.f / (1.f + expf(-bv)) : expf(bv - big);
+            if (scoring != DMM_SCORE_SIGMOID) w[t * k + n] = expf(bv - big);
+            else if (normalize) w[t * k + n] = expf(fminf(bv, 0.f) - fminf(big, 0.f)) / (1.f + expf(-fabsf(bv)));
+            else w[t * k + n] = 1.f / (1.f + expf(-bv));
             of[best + 1]++;
         }
         if (normalize) {

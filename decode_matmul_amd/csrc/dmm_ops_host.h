@@ -4,7 +4,10 @@
 inline bool type_ok(int t) { return t == DMM_F16 || t == DMM_F32; }
 inline uintptr_t type_bytes(int t) { return t == DMM_F32 ? 4 : 2; }
 
-// what both products ask of their arguments; on_y: rows of y, codes: E matrices
+// rows of x and of y in one call: row numbers of a tile that begins at the last row stay below 2^31
+constexpr int64_t kOpsMaxRows = 1 << 30;
+
+// what both products ask of their arguments: T rows of x, R rows of y, E matrices
 int check_ops(const void *x, int64_t T, const void *codes, const void *grid, const dmm_epilogue *ep, const void *y, int64_t R,
               int64_t E, int64_t N, int64_t K)
 {
@@ -20,7 +23,7 @@ int check_ops(const void *x, int64_t T, const void *codes, const void *grid, con
         (ep->bias && !aligned(ep->bias, type_bytes(ep->bias_type))) ||
         (ep->residual && !aligned(ep->residual, type_bytes(ep->residual_type))))
         return DMM_ERR_MISALIGNED;
-    if (T > INT32_MAX || R > INT32_MAX || E > 65535 || N > INT32_MAX / 2 || K > INT32_MAX) return DMM_ERR_TOO_LARGE;
+    if (T > kOpsMaxRows || R > kOpsMaxRows || E > 65535 || N > INT32_MAX / 2 || K > INT32_MAX) return DMM_ERR_TOO_LARGE;
     return DMM_OK;
 }
 
@@ -84,13 +87,13 @@ int run_ops_gemm(const void *x, const void *codes, const void *grid, const Group
 std::atomic<int> g_ops_kernel{-1};
 enum OpsKernel { kOpsGeneric = 0, kOpsRows = 1, kOpsGemm = 2, kOpsSplit = 3, kOpsRows8 = 4, kOpsMid = 5 };
 
-template <int NT, int XI, int W, int CG, bool kGated, bool kOne>
+template <int NT, int XI, int W, int CG, bool kGated, bool kOne, int D = 2>
 int launch_ops_rows_inst(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, int64_t units,
                          hipStream_t s)
 {
     const int64_t wgs = units < cu_count() ? units : cu_count();
     const OpsRowsArgs args{(const uint16_t *)x, (const uint16_t *)codes, grid, g, e, (int)K, (int)(units / wgs), (int)(units % wgs)};
-    return launch(ops_rows_kernel<NT, 2, XI, W, CG, kGated, kOne>, dim3((unsigned)wgs), dim3(64 * W), (size_t)fd_lds_bytes(XI, W), s, args);
+    return launch(ops_rows_kernel<NT, D, XI, W, CG, kGated, kOne>, dim3((unsigned)wgs), dim3(64 * W), (size_t)fd_lds_bytes(XI, W), s, args);
 }
 
 // most segments the rows can make, sr rows each: an expert adds at most one cut one, and none without a row
@@ -98,6 +101,13 @@ inline int64_t ops_segments(const Groups &g, int64_t sr)
 {
     const int64_t full = ((int64_t)g.R + sr - 1) / sr;
     return g.offsets ? std::min<int64_t>((int64_t)g.R, (int64_t)g.R / sr + g.E) : full;
+}
+
+// Whether the jobs of a call can be counted in 31 bits, whatever the list of the experts' rows holds: one that does
+// not increase may give every expert all rows.
+inline bool ops_jobs_fit(const Groups &g, int64_t sr, int64_t N)
+{
+    return (g.offsets ? (int64_t)g.E : 1) * (((int64_t)g.R + sr - 1) / sr) * ((N + 15) / 16) < (1LL << 31);
 }
 
 template <int XI, int W, int CG, bool kGated>
@@ -110,8 +120,14 @@ int launch_ops_rows(const void *x, const void *codes, const void *grid, const Gr
         if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated, true>(x, codes, grid, g, e, K, units, s);
         return launch_ops_rows_inst<8, XI, W, CG, kGated, true>(x, codes, grid, g, e, K, units, s);
     }
-    if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
-    if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
+    if constexpr (XI != 4) {   // four to eight rows: dense, one segment; not here with so few tiles
+        if (share <= 2) return launch_ops_rows_inst<2, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
+        if (share <= 4) return launch_ops_rows_inst<4, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
+    }
+    // Eight waves, gated: four code loads in flight per wave where a job has more than one step per wave (2 x 11008 x 4096, 8
+    // experts, 40 rows 58.5 us with two, 54.6 with four; but 2 x 1408 x 2048, 64 experts, 128 rows 27.5 / 29.2; not gated no difference)
+    if constexpr (kGated && W == 8 && CG == 1)
+        if (K > 2048) return launch_ops_rows_inst<8, XI, W, CG, kGated, false, 4>(x, codes, grid, g, e, K, units, s);
     return launch_ops_rows_inst<8, XI, W, CG, kGated, false>(x, codes, grid, g, e, K, units, s);
 }
 
@@ -227,7 +243,7 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
     if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
-    const bool rows_ok = ops_segments(g, 2) * ((e.N + 15) / 16) < (1LL << 31);
+    const bool rows_ok = ops_jobs_fit(g, 4, e.N), mid_ok = ops_jobs_fit(g, kMidRows, e.N);
     const int cus = cu_count();
     // One row of a matrix: the batch-1 kernels' bodies
     const bool one_row = force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0;
@@ -238,14 +254,14 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     // the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7 us, 16-bit 14.4; 2 rows 18.9 / 21.1; but 4 rows 24.7 / 20.6).  A
     // job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored twice,
     // which a residual that is the output itself would not survive.
-    const bool rows8_ok = rows_ok && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cus);
+    const bool rows8_ok = ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cus);
     const bool rows8_pays = g.offsets ? (g.R <= 2 || 4 * (int64_t)g.R <= g.E) && K >= 4096 &&
                                             std::min<int64_t>(g.R, g.E) * rows * (K >> 2) >= (20LL << 20)
                                       : g.R <= 2;
     if (rows8_ok && (force == kOpsRows8 || (force < 0 && rows8_pays && gemv_q8_enabled())))
         return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && force == kOpsRows) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
-    if (rows_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
+    if (mid_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
     if (g.offsets) {
         // Up to eight rows per expert the few-rows kernel, up to 160 the one for tens of rows where every wave has a unit
         // (graph launches, us, few rows / tens / matrix-matrix, rows per expert: 2 x 11008 x 4096, 8 experts 6: 58 / 66 / 88, 12: 77 / 68 /
@@ -254,7 +270,7 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
         // 299 / 273; but 4096 x 4096, 8 experts, 8 units per workgroup, 12: 20 / 24)
         const int64_t avg = g.R / g.E, units = (int64_t)g.E * ((avg + 31) / 32) * ((e.N + 15) / 16);
         if (force < 0 && rows_ok && (avg < 8 || (avg <= 64 && units <= 8LL * cus))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
-        if (force < 0 && rows_ok && avg < 160) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
+        if (force < 0 && mid_ok && avg < 160) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
         return run_ops_gemm<kGated>(x, codes, grid, g, e, K, s);
     }
     if (force < 0 && rows_ok && ops_rows_beat_split(g.R, e.N, K, kGated, cus)) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
@@ -297,12 +313,18 @@ const std::vector<KernelInfo> &ops_kernel_table()
         DMM_K_OPS(false), DMM_K_OPS(true),
 #undef DMM_K_OPS
 #define DMM_K_ROWS_X(NT, G, O)                                                                                                    \
-    kinfo(ops_rows_kernel<NT, 2, 2, 16, 1, G, O>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 4, 16, 1, G, O>, kLdsMax, true),   \
-        kinfo(ops_rows_kernel<NT, 2, 8, 8, 1, G, O>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 8, 8, 2, G, O>, kLdsMax, true)
+    kinfo(ops_rows_kernel<NT, 2, 2, 16, 1, G, O>, kLdsMax, true), kinfo(ops_rows_kernel<NT, 2, 8, 8, 1, G, O>, kLdsMax, true),    \
+        kinfo(ops_rows_kernel<NT, 2, 8, 8, 2, G, O>, kLdsMax, true)
 #define DMM_K_ROWS(G, O) DMM_K_ROWS_X(2, G, O), DMM_K_ROWS_X(4, G, O), DMM_K_ROWS_X(8, G, O)
         DMM_K_ROWS(false, false), DMM_K_ROWS(true, false), DMM_K_ROWS(false, true), DMM_K_ROWS(true, true),
 #undef DMM_K_ROWS
 #undef DMM_K_ROWS_X
+        kinfo(ops_rows_kernel<8, 4, 8, 8, 1, true, false>, kLdsMax, true),
+#define DMM_K_ROWS_4(G)                                                                                                           \
+    kinfo(ops_rows_kernel<2, 2, 4, 16, 1, G, true>, kLdsMax, true), kinfo(ops_rows_kernel<4, 2, 4, 16, 1, G, true>, kLdsMax, true), \
+        kinfo(ops_rows_kernel<8, 2, 4, 16, 1, G, true>, kLdsMax, true), kinfo(ops_rows_kernel<8, 2, 4, 16, 1, G, false>, kLdsMax, true)
+        DMM_K_ROWS_4(false), DMM_K_ROWS_4(true),
+#undef DMM_K_ROWS_4
 #define DMM_K_OQ8D(G)                                                                                                             \
     kinfo(ops_q8d_kernel<2, 1, 2, G>, kLdsMax, true), kinfo(ops_q8d_kernel<4, 1, 2, G>, kLdsMax, true),                           \
         kinfo(ops_q8d_kernel<6, 1, 3, G>, kLdsMax, true), kinfo(ops_q8d_kernel<8, 1, 2, G>, kLdsMax, true)
@@ -439,7 +461,7 @@ int check_route(const void *logits, int type, int64_t T, int64_t E, int64_t k, i
     if (T < 0 || E < 1 || k < 1 || k > E) return DMM_ERR_BAD_SHAPE;
     if (type != DMM_F16 && type != DMM_F32 && type != DMM_BF16) return DMM_ERR_BAD_SHAPE;
     if (scoring != DMM_SCORE_SOFTMAX && scoring != DMM_SCORE_SIGMOID) return DMM_ERR_BAD_SHAPE;
-    if (E > kRouteMaxE || k > kRouteMaxK || T * k > INT32_MAX) return DMM_ERR_TOO_LARGE;
+    if (E > kRouteMaxE || k > kRouteMaxK || T > kRouteMaxT || T * k > INT32_MAX) return DMM_ERR_TOO_LARGE;
     if (!offsets || (T > 0 && (!logits || !weights || !experts || !rows || !slots))) return DMM_ERR_NULL_POINTER;
     if (!aligned(logits, type_bytes(type)) || !aligned(weights, 4) || !aligned(experts, 4) || !aligned(offsets, 4) || !aligned(rows, 4) ||
         !aligned(slots, 4))

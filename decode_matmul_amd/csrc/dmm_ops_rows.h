@@ -99,7 +99,7 @@ __device__ __forceinline__ bool ops_range(const Groups &g, const GroupRange &fir
         }
     }
     parts = (uint32_t)uniform((int)parts);
-    const uint32_t jobs = (uint32_t)segs * parts;   // below 2^31 (the host's business)
+    const uint32_t jobs = (uint32_t)segs * parts;   // below 2^31 (ops_jobs_fit)
     const uint32_t b = blockIdx.x, q = jobs / wgs, rest = jobs - q * wgs;
     const uint32_t j0 = b * q + (b < rest ? b : rest);
     c.left = (int)(q + (b < rest ? 1u : 0u));
@@ -592,6 +592,6 @@ struct Q8dOps {
 template <int NT, int U, int D, bool kGated>
 __global__ __launch_bounds__(1024) void ops_q8d_kernel(OpsRowsArgs args)
 {
-    const Q8dOps<NT < 2 ? 2 : NT, kGated> p{args};
+    const Q8dOps<NT, kGated> p{args};
     gemv_q8d_body<NT, U, D, false>(p, args.x, args.codes, args.grid, args.epi.N, args.K, args.units_q, args.units_r);
 }

@@ -14,7 +14,9 @@
 // order of ors does not matter, so the result does not depend on it); a place inside the block is a population count.
 // The masks and their counts go to the workspace and a second kernel adds the counts of the blocks before; with one
 // block the same launch does it all.
+// Every block of the second kernel reads the counts of all blocks, which sets the limit on the tokens of a call.
 constexpr int kRouteMaxE = 1024, kRouteMaxK = 64;
+constexpr int64_t kRouteMaxT = 1 << 24;
 
 __device__ __forceinline__ uint32_t route_key(float v)
 {
@@ -138,14 +140,16 @@ __device__ __forceinline__ int route_token(const RouteArgs &a, const RouteRow<EV
         }
     }
     // weights.  softmax: exp(v - largest) over the sum of the chosen ones, or of the whole row; a NaN anywhere in the
-    // row shows in all its weights
+    // row shows in all its weights.  sigmoid over the sum of the chosen ones: exp(v) / (1 + exp(v)) = exp(min(v, 0)) /
+    // (1 + exp(-|v|)), numerators relative to the largest choice's, so that a row of very low logits does not end in 0 / 0.
     float w, total = 1.f;
     uint32_t bad = 0;
 #pragma unroll
     for (int i = 0; i < EV; i++) bad |= v[i] != v[i] ? 1u : 0u;
     bad = lanes_reduce<L>(bad, OrU32());
     if (a.sigmoid) {
-        w = mine >= 0 ? epi_sigmoid(val) : 0.f;
+        if (a.normalize) w = mine >= 0 ? expf(fminf(val, 0.f) - fminf(big, 0.f)) / (1.f + expf(-fabsf(val))) : 0.f;
+        else w = mine >= 0 ? epi_sigmoid(val) : 0.f;
     } else {
         w = mine >= 0 ? expf(val - big) : 0.f;
         if (!a.normalize) {

@@ -352,6 +352,12 @@ torch::Tensor decode_matmul_fused(torch::Tensor x, torch::Tensor codes, torch::T
     return y;
 }
 
+bool share_memory(const torch::Tensor &a, const torch::Tensor &b)   // both contiguous
+{
+    const char *pa = static_cast<const char *>(a.data_ptr()), *pb = static_cast<const char *>(b.data_ptr());
+    return a.nbytes() > 0 && b.nbytes() > 0 && pa < pb + b.nbytes() && pb < pa + a.nbytes();
+}
+
 torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch::Tensor grid, double scale, MaybeTensor scales,
                                     torch::Tensor offsets, MaybeTensor rows, MaybeTensor bias, const std::string &activation,
                                     bool gated, torch::ScalarType out_dtype, MaybeTensor out)
@@ -380,8 +386,8 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
     if (scales) {
         DMM_CHECK_SAME_DEVICE(*scales, x.device());
         DMM_CHECK_CONTIGUOUS(*scales);
-        TORCH_CHECK(scales->scalar_type() == torch::kFloat && scales->size(0) == E &&
-                        (scales->dim() == 1 || (gated && scales->dim() == 2 && scales->size(1) == 2)),
+        TORCH_CHECK(scales->scalar_type() == torch::kFloat &&
+                        (scales->dim() == 1 || (gated && scales->dim() == 2 && scales->size(1) == 2)) && scales->size(0) == E,
                     "scale must be a number, float32 [E], or float32 [E, 2] for a gated call");
         check_no_grad(*scales, "decode_matmul_grouped", "scale");
         scale_cols = static_cast<int>(scales->dim());
@@ -403,6 +409,8 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
         TORCH_CHECK(out->dim() == 2 && out->size(0) == R && out->size(1) == N && out->scalar_type() == out_dtype,
                     "out must be [R, N] of out_dtype");
         check_no_grad(*out, "decode_matmul_grouped", "out");
+        for (const torch::Tensor *t : {&x, &codes, &grid, &offsets, rows ? &*rows : nullptr, scales ? &*scales : nullptr, bias ? &*bias : nullptr})
+            TORCH_CHECK(!t || !share_memory(*out, *t), "out must not share memory with an input");
         y = *out;
     } else {
         y = torch::empty({R, N}, x.options().dtype(out_dtype).requires_grad(false));
@@ -443,6 +451,7 @@ std::vector<torch::Tensor> route_experts(torch::Tensor logits, int64_t k, const 
     const int type = logits.scalar_type() == torch::kBFloat16 ? DMM_BF16 : float_type(logits, "logits must be bfloat16, or");
     const int64_t T = logits.size(0), E = logits.size(1);
     TORCH_CHECK(k >= 1 && k <= E && k <= 64 && E <= 1024, "k must be between 1 and min(E, 64), and E at most 1024");
+    TORCH_CHECK(T <= 1 << 24 && T * k <= INT32_MAX, "at most 2^24 tokens per call");
     const int sc = scoring == "sigmoid" ? DMM_SCORE_SIGMOID : DMM_SCORE_SOFTMAX;
     c10::OptionalDeviceGuard guard;
     if (logits.is_cuda()) guard.reset_device(logits.device());

@@ -292,7 +292,8 @@ enum { DMM_ACT_NONE = 0, DMM_ACT_RELU = 1, DMM_ACT_SILU = 2, DMM_ACT_GELU = 3, D
  *   z = scale * sum + bias;   y = act(z)                          gated == 0: W has N rows
  *   y = act(z[n]) * z[N + n]                                      gated != 0: W has 2 N rows, gate then up
  *   y += residual
- * Types are DMM_F16 or DMM_F32; a NULL bias or residual is left out and its type not looked at. */
+ * Types are DMM_F16 or DMM_F32; a NULL bias or residual is left out and its type not looked at.  y may be the residual
+ * itself and shares memory with no other input. */
 typedef struct dmm_epilogue {
     const void *bias;        /* [N], gated [2 N] (grouped: one such row per expert)       */
     const void *residual;    /* [M, N]; may be y itself.  dmm_decode_matmul_grouped: NULL  */
@@ -321,7 +322,8 @@ int dmm_decode_matmul_fused(const void *x, const void *codes, const void *grid, 
  *            stands for a row of zeros.
  *   scales   float [E] on the device, times the epilogue's scale and scale_up; scale_cols == 2 (gated only):
  *            [E,2], gate and up; or NULL.
- * Rows of y that belong to no expert (from offsets[E] on) are left as they were.  Up to 65535 experts. */
+ * Rows of y that belong to no expert (from offsets[E] on) are left as they were.  Up to 65535 experts.
+ * Both products take up to 2^30 rows of x and of y; more are refused with DMM_ERR_TOO_LARGE. */
 int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const void *codes, const void *grid,
                               const void *scales, int scale_cols, const void *offsets,
                               const dmm_epilogue *epilogue, void *y, int64_t R, int64_t E, int64_t N, int64_t K,
@@ -345,7 +347,7 @@ int dmm_set_ops_kernel(int kernel);
  *            dmm_decode_matmul_grouped takes
  *   slots    int32 [T,k]: the sorted row of every choice, -1 for one that was not made; what
  *            dmm_combine_experts takes
- * E <= 1024, k <= min(E, 64).  The workspace (16-byte aligned, dmm_route_workspace_bytes, 0 up to 64 tokens) is needed
+ * T <= 2^24, E <= 1024, k <= min(E, 64).  The workspace (16-byte aligned, dmm_route_workspace_bytes, 0 up to 64 tokens) is needed
  * whole: fewer bytes are refused with DMM_ERR_SCRATCH_TOO_SMALL. */
 enum { DMM_SCORE_SOFTMAX = 0, DMM_SCORE_SIGMOID = 1 };
 int64_t dmm_route_workspace_bytes(int64_t T, int64_t E);
@@ -355,7 +357,8 @@ int dmm_route_experts(const void *logits, int logits_type, int64_t T, int64_t E,
 
 /* The weighted sum of the experts' rows: out[t] = residual[t] + sum over j, in order, of weights[t,j] * y[slots[t,j]], in fp32
  * with one rounding; y [R,N] and out [T,N] half or float, weights float [T,k], slots int32 [T,k].  A slot outside
- * 0 .. R - 1 adds nothing.  residual [T,N] half or float, or NULL; it may be out itself. */
+ * 0 .. R - 1 adds nothing.  residual [T,N] half or float, or NULL; it may be out itself.  out shares memory with no
+ * other input. */
 int dmm_combine_experts(const void *y, int y_type, const void *slots, const void *weights, const void *residual,
                         int residual_type, void *out, int out_type, int64_t R, int64_t T, int64_t k, int64_t N,
                         void *stream);

@@ -275,6 +275,34 @@ def test_route(T, E, k, dtype, scoring, normalize):
     check_routing(dmm.route_experts(logits.to(DEV), k, scoring=scoring, normalize=normalize), logits, k, scoring, normalize)
 
 
+def test_route_sigmoids_too_small_for_a_float_still_have_shares():
+    gen = torch.Generator().manual_seed(7)
+    for E, k in ((9, 4), (300, 20)):
+        z = torch.randn(6, E, generator=gen) * 5 - torch.tensor([0.0, 60, 90, 200, 400, 600]).view(6, 1)
+        check_routing(dmm.route_experts(z.to(DEV), k, scoring="sigmoid"), z, k, "sigmoid", True)
+    for dtype in (F16, F32, torch.bfloat16):
+        w = dmm.route_experts(torch.full((2, 5), torch.finfo(dtype).min, dtype=dtype, device=DEV), 4, scoring="sigmoid").weights
+        assert torch.equal(w.cpu(), torch.full((2, 4), 0.25))
+
+
+def test_grouped_lists_that_give_every_expert_all_rows(kernel):
+    """A list that does not increase: rows of several experts, written by each of them; every one stays inside y."""
+    R, E, N, K = 70, 40, 52, 320
+    x, codes, grid, _, rows, _ = grouped_inputs((2,) * 35 + (0,) * 5, 9, N, K, True, None, True, seed=5, coarse=True)
+    out = torch.zeros(R + 2, N, dtype=F16, device=DEV)
+    broken = torch.tensor(([0, R] * E)[:E + 1], dtype=torch.int32, device=DEV)
+    dmm.decode_matmul_grouped(*dev(x, codes, grid), 0.1, broken, rows=rows.to(DEV), gated=True, out=out[1:R + 1])
+    torch.cuda.synchronize()
+    assert torch.all(out[0] == 0) and torch.all(out[-1] == 0)
+    # which matrix gives an element its value is not said: one of those whose range is not empty.  Both sides are rounded once
+    # (2 x 2^-11); the fp32 sums of a few hundred products, of either order, are far nearer than 1e-3.
+    got, near = out[1:R + 1].float(), torch.zeros(R, N, dtype=torch.bool, device=DEV)
+    for c in codes.to(DEV)[::2]:
+        want = dmm.decode_matmul_fused(x.to(DEV)[rows.to(DEV).long()], c, grid.to(DEV), 0.1, gated=True).float()
+        near |= (got - want).abs() <= 2.0 ** -10 * want.abs() + 1e-3
+    assert near.all()
+
+
 def test_route_many_tokens_against_the_host_route():
     """More than one block, one and several words per expert's mask; the lists equal the host's bit for bit."""
     for T, E, k in ((5000, 16, 2), (33000, 40, 3), (140000, 8, 2)):

@@ -104,6 +104,10 @@ def test_grouped_refusals():
         f(x, codes, grid, 1.0, offsets, rows=rows, out=torch.empty(5, 7, dtype=F16))
     with pytest.raises(RuntimeError, match="out must be"):
         f(x, codes, grid, 1.0, offsets, rows=rows, out=torch.empty(5, 8, dtype=F16), out_dtype=F32)
+    with pytest.raises(RuntimeError, match="share memory"):
+        f(x, codes, grid, 1.0, offsets, rows=rows, out=x.view(-1)[200:240].view(5, 8))
+    with pytest.raises(RuntimeError, match="scale"):
+        f(x, codes, grid, torch.ones(()), offsets, rows=rows)
     with pytest.raises(RuntimeError, match="gradient"):
         f(x, codes, grid, torch.ones(2, requires_grad=True), offsets, rows=rows)
 
@@ -131,6 +135,15 @@ def test_route_zeros_of_both_signs_are_equal_and_nan_shows():
     assert torch.isnan(r.weights[0]).all() and torch.isfinite(r.weights[1]).all()
 
 
+def test_route_sigmoids_too_small_for_a_float_still_have_shares():
+    gen = torch.Generator().manual_seed(7)
+    z = torch.randn(6, 9, generator=gen) * 5 - torch.tensor([0.0, 60, 90, 200, 400, 600]).view(6, 1)
+    check_routing(dmm.route_experts(z, 4, scoring="sigmoid"), z, 4, "sigmoid", True)
+    for dtype in (F16, F32, torch.bfloat16):        # a row that a mask of the type's lowest value covers: equal shares
+        w = dmm.route_experts(torch.full((2, 5), torch.finfo(dtype).min, dtype=dtype), 4, scoring="sigmoid").weights
+        assert torch.equal(w, torch.full((2, 4), 0.25))
+
+
 def test_route_refusals():
     z = torch.zeros(3, 8)
     for k in (0, 9, -1):
@@ -144,6 +157,8 @@ def test_route_refusals():
         dmm.route_experts(z.double(), 2)
     with pytest.raises(RuntimeError, match="contiguous"):
         dmm.route_experts(z.t(), 2)
+    with pytest.raises(RuntimeError, match="tokens"):
+        dmm.route_experts(torch.zeros(2 ** 24 + 1, 1, dtype=F16), 1)
     with pytest.raises(RuntimeError, match="gradient"):
         dmm.route_experts(z.requires_grad_(), 2)
 
@@ -205,6 +220,7 @@ def test_status_codes_of_the_operators_around_the_product():
     assert fused(p, p, p, ep(activation=5), p, 1, 4, 16, None, 0, None) == -2
     assert fused(p, p, p, ep(out_type=2), p, 1, 4, 16, None, 0, None) == -2  # bfloat16 is for logits only
     assert fused(p, p, p, ep(), p, 1, 1 << 31, 16, None, 0, None) == -4
+    assert fused(p, p, p, ep(), p, (1 << 30) + 1, 4, 16, None, 0, None) == -4
     assert fused(p, p, p, ep(), p, 1, 4, 16, ctypes.c_void_p(p.value + 4), 64, None) == -3
     assert fused(p, p, p, ep(), p, 1, 4, 16, p, -1, None) == -2
     assert fused(None, None, None, ep(), None, 0, 4, 16, None, 0, None) == 0
@@ -215,6 +231,8 @@ def test_status_codes_of_the_operators_around_the_product():
     assert grouped(p, 3, p, p, p, None, 1, None, ep(), p, 4, 2, 4, 16, None) == -1
     assert grouped(p, 3, p, p, p, None, 1, odd, ep(), p, 4, 2, 4, 16, None) == -3
     assert grouped(p, 3, p, p, p, None, 1, p, ep(), p, 4, 65536, 4, 16, None) == -4
+    assert grouped(p, 3, p, p, p, None, 1, p, ep(), p, (1 << 30) + 1, 2, 4, 16, None) == -4
+    assert grouped(p, (1 << 30) + 1, p, p, p, None, 1, p, ep(), p, 4, 2, 4, 16, None) == -4
     assert grouped(None, 0, None, None, None, None, 1, None, ep(), None, 0, 2, 4, 16, None) == 0
     route = lib.dmm_route_experts
     assert route(p, 1, 3, 8, 9, 0, 1, p, p, p, p, p, None, 0, None) == -2
@@ -223,6 +241,7 @@ def test_status_codes_of_the_operators_around_the_product():
     assert route(p, 1, 3, 2000, 2, 0, 1, p, p, p, p, p, None, 0, None) == -4
     assert route(p, 1, 3, 8, 2, 0, 1, p, p, None, p, p, None, 0, None) == -1
     assert route(p, 1, 3, 8, 2, 0, 1, odd, p, p, p, p, None, 0, None) == -3
+    assert route(p, 1, (1 << 24) + 1, 8, 2, 0, 1, p, p, p, p, p, None, 0, None) == -4
     need = lib.dmm_route_workspace_bytes(100, 8)
     assert need > 0 and lib.dmm_route_workspace_bytes(64, 8) == 0 and lib.dmm_route_workspace_bytes(-1, 8) == 0
     assert route(p, 1, 100, 8, 2, 0, 1, p, p, p, p, p, None, 0, None) == -1
