@@ -81,13 +81,13 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
         }
     };
     const uint32_t xs = lds_addr(smem_raw) + (uint32_t)kSTablesBytes;
-    // row 8 i + wave: 16 bytes of piece `lane` in slot lane ^ (row % 16)
-    const uint32_t xs_w0 = xs + (uint32_t)(wave * 1024 + ((lane ^ wave) << 4)), xs_w1 = xs + (uint32_t)(wave * 1024 + ((lane ^ (wave + 8)) << 4));
+    // row 8 i + wave: 16 bytes of piece `lane` in slot x_slot(lane) ^ (row % 16)
+    const uint32_t xs_w0 = xs + (uint32_t)(wave * 1024 + ((x_slot(lane) ^ wave) << 4)), xs_w1 = xs + (uint32_t)(wave * 1024 + ((x_slot(lane) ^ (wave + 8)) << 4));
     auto store_x = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < 4; i++) lds_write16(((i & 1) ? xs_w1 : xs_w0) + (uint32_t)(buf * kMidXBuf + i * 8192), xv[i]);
     };
-    const uint32_t xs_r = xs + (uint32_t)(c16 * 1024 + (((8 * q) ^ c16) << 4));
+    const uint32_t xs_r = xs + (uint32_t)(c16 * 1024 + ((x_slot(8 * q) ^ c16) << 4));
 
     const int voff = c16 * row_bytes + q * 16;
     u4_t cw[NT];

@@ -61,6 +61,11 @@ __device__ __forceinline__ GroupRange ops_first_ranges(const Groups &g, int lane
     return first;
 }
 
+// Where 16-byte piece p of a step of x lies in its row (before the exchange by the row's number): pieces 8 .. 15 behind 16 .. 23.
+// A 16-byte LDS read is served sixteen lanes at a time, half of them of one quarter of the wave and half of the next; the
+// two read pieces 8 apart, which must not differ in the bank then.
+__device__ __forceinline__ int x_slot(int p) { return (p & ~24) | (p >> 1 & 8) | (p << 1 & 16); }
+
 // the workgroup's range of jobs; false: it has none
 template <int SR, int NU, int kFixed>
 __device__ __forceinline__ bool ops_range(const Groups &g, const GroupRange &first, int upn, int lane, OpsCursor &c)
@@ -318,11 +323,11 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
             }
         }
     };
-    // the wave's piece, addressed as in gemv_f16d_kernel
+    // the wave's piece: row m at a pitch of 512 bytes, its pieces exchanged by m
     const uint32_t piece = lds_addr(smem_raw) + (uint32_t)(kSTablesBytes + wave * kPiece);
-    auto xs_w = [&]() { return piece + (uint32_t)((lane >> 5) * 512 + (((lane & 31) ^ (lane >> 5)) << 4)); };
+    auto xs_w = [&]() { return piece + (uint32_t)((lane >> 5) * 512 + ((x_slot(lane & 31) ^ (lane >> 5)) << 4)); };
     const int xr_row = c16 & (CM - 1);
-    const uint32_t xs_r = piece + (uint32_t)(xr_row * 512 + (((8 * q) ^ xr_row) << 4));
+    const uint32_t xs_r = piece + (uint32_t)(xr_row * 512 + ((x_slot(8 * q) ^ xr_row) << 4));
 
     const int voff = c16 * row_bytes + q * 16;
     auto issue = [&](u4_t &cwd, const OpsItem &it, int t) {
