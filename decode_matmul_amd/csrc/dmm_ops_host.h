@@ -264,10 +264,10 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     if (mid_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
     if (g.offsets) {
         // Up to eight rows per expert the few-rows kernel, up to 160 the one for tens of rows where every wave has a unit
-        // (graph launches, us, few rows / tens / matrix-matrix, rows per expert: 2 x 11008 x 4096, 8 experts 6: 58 / 66 / 88, 12: 77 / 68 /
-        // 90, 31: 126 / 98 / 180, 64: 222 / 165 / 218, 128: - / 288 / 361, 256: - / 529 / 534; 4096 x 11008, 16 experts 8: 73 / 75 / 141, 31: 113 / 98 /
-        // 147, 128: - / 287 / 291, 256: - / 541 / 451; 2 x 1408 x 2048, 64 experts 8: 44 / 47 / 66, 31: 94 / 68 / 98, 128: - / 163 / 196, 256: - /
-        // 299 / 273; but 4096 x 4096, 8 experts, 8 units per workgroup, 12: 20 / 24)
+        // (graph launches, us, few rows / tens / matrix-matrix, rows per expert: 2 x 11008 x 4096, 8 experts 4: 56 / 62 / 88, 8: 75 / 68 /
+        // 90, 31: 127 / 92 / 181, 64: 224 / 165 / 221, 128: - / 288 / 367, 256: - / 528 / 533; 4096 x 11008, 16 experts 4: 50 / 63 / 74,
+        // 8: 74 / 73 / 141, 31: 114 / 100 / 147, 128: - / 288 / 292, 256: - / 533 / 455; 2 x 1408 x 2048, 64 experts 4: 33 / 37 / 51, 8: 47 /
+        // 46 / 66, 31: 93 / 65 / 99, 128: - / 159 / 196, 256: - / 294 / 274; but 4096 x 4096, 8 experts, 8 units per workgroup, 12: 20 / 24)
         const int64_t avg = g.R / g.E, units = (int64_t)g.E * ((avg + 31) / 32) * ((e.N + 15) / 16);
         if (force < 0 && rows_ok && (avg < 8 || (avg <= 64 && units <= 8LL * cus))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
         if (force < 0 && mid_ok && avg < 160) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
