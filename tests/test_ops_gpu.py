@@ -452,3 +452,40 @@ def test_mixed_devices_are_refused():
         dmm.decode_matmul_fused(*dev(x, codes, grid), 1.0, bias=b)
     with pytest.raises(RuntimeError, match="same device"):
         dmm.combine_experts(torch.zeros(2, 8, dtype=F16, device=DEV), torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, 1, device=DEV))
+
+
+# ----------------------------------------------------------------- past 32 bits
+def test_grouped_codes_past_4_gib(kernel):
+    E, N, K = 2100, 1024, 8192                                     # 2 MiB of codes per expert
+    who, counts = [0, 1049, E - 1], (5, 40, 25)
+    x, some, grid, ends, rows, b = grouped_inputs(counts, 9, N, K, False, F32, True, seed=4, coarse=kernel == 4)
+    codes = torch.zeros(E, N, K // 8, dtype=torch.int16, device=DEV)
+    bias = torch.zeros(E, N, dtype=F32, device=DEV)
+    sizes = torch.zeros(E, dtype=torch.int64)
+    for i, e in enumerate(who):
+        codes[e], bias[e], sizes[e] = some[i].to(DEV), b[i].to(DEV), counts[i]
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), sizes.cumsum(0)]).int()
+    y = dmm.decode_matmul_grouped(x.to(DEV), codes, grid.to(DEV), 0.01, offsets.to(DEV), rows=rows.to(DEV), bias=bias)
+    assert_within(y, *grouped64(x, some, grid, 0.01, ends, rows, b, False, "none", F16, N))
+
+
+@pytest.mark.parametrize("kernel", [-1, 0, 1, 5])
+def test_results_past_4_gib(kernel):
+    M, N, K = 70000, 32768, 64
+    x, codes, grid, _, _ = fused_inputs(M, N, K, False, None, None, 6)
+    lib = capi.lib()
+    lib.dmm_set_ops_kernel(kernel)
+    try:
+        y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.1, activation="relu")
+        torch.cuda.synchronize()
+    finally:
+        lib.dmm_set_ops_kernel(-1)
+    pick = torch.tensor([0, 1, 35000, 65535, 65536, 69997, 69999])
+    want, tol = product64(x[pick].double(), decode64(codes, grid), (0.1, 0.1), None, False, "relu", None, F16)
+    assert_within(y[pick.to(DEV)], want, tol)
+    slots = torch.tensor([[M - 1, 65536], [0, M - 2], [M, 35000]], dtype=torch.int32)
+    w = torch.tensor([[0.5, 0.25], [1.5, -1.0], [3.0, 2.0]])
+    got = dmm.combine_experts(y, slots.to(DEV), w.to(DEV))
+    near = torch.tensor([[0, 1], [2, 3], [9, 4]], dtype=torch.int32)            # the same rows in a small y
+    few = y[torch.tensor([M - 1, 65536, 0, M - 2, 35000]).to(DEV)].cpu()
+    assert_within(got, *combine64(few, near, w, None, F16))
