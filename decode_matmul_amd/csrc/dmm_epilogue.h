@@ -14,7 +14,6 @@ struct Epi {
     int act;
     int scale_cols;
     int bias_f32, residual_f32, out_f32;
-    int vec;                // N % 4 == 0 and every pointer aligned for four elements at a time
 };
 
 // 1 / (1 + exp(-z)) to about two units in the last place.  exp(-z) = 2^t (1 + ln 2 * r) with t the rounded product
@@ -49,12 +48,46 @@ __device__ __forceinline__ float epi_load(const void *p, int64_t i, int f32)
     return f32 ? reinterpret_cast<const float *>(p)[i] : (float)reinterpret_cast<const half_t *>(p)[i];
 }
 
-// four elements from i on, i % 4 == 0 and p aligned (Epi::vec)
-__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32)
+// Four elements at a time, wherever a row starts: global loads and stores need no more than the element's alignment.
+struct __attribute__((packed, aligned(2))) H4Any {
+    h4_t v;
+};
+struct __attribute__((packed, aligned(4))) F4Row {
+    f4_t v;
+};
+
+// elements i .. i + 3, zeros from the left-th on
+__device__ __forceinline__ f4_t epi_load4(const void *p, int64_t i, int f32, int left)
 {
-    if (f32) return *reinterpret_cast<const f4_t *>(reinterpret_cast<const float *>(p) + i);
-    const h4_t h = *reinterpret_cast<const h4_t *>(reinterpret_cast<const half_t *>(p) + i);
+    if (__builtin_expect(left < 4, 0)) {
+        f4_t r = f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            if (k < left) r[k] = epi_load(p, i + k, f32);
+        return r;
+    }
+    if (f32) return reinterpret_cast<const F4Row *>(reinterpret_cast<const float *>(p) + i)->v;
+    const h4_t h = reinterpret_cast<const H4Any *>(reinterpret_cast<const half_t *>(p) + i)->v;
     return f4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+}
+
+__device__ __forceinline__ void epi_put4(void *p, int64_t i, int f32, int left, f4_t z)
+{
+    if (__builtin_expect(left < 4, 0)) {
+#pragma unroll
+        for (int k = 0; k < 3; k++)
+            if (k < left) {
+                if (f32) reinterpret_cast<float *>(p)[i + k] = z[k];
+                else reinterpret_cast<half_t *>(p)[i + k] = (half_t)z[k];
+            }
+    } else if (f32) {
+        reinterpret_cast<F4Row *>(reinterpret_cast<float *>(p) + i)->v = z;
+    } else {
+        h4_t h;
+#pragma unroll
+        for (int k = 0; k < 4; k++) h[k] = (half_t)z[k];
+        reinterpret_cast<H4Any *>(reinterpret_cast<half_t *>(p) + i)->v = h;
+    }
 }
 
 struct EpiScale {
@@ -116,59 +149,52 @@ __device__ __forceinline__ f4_t epi_act4(f4_t z, int act)
     return z;
 }
 
-// What the epilogue of four outputs (row, n .. n + 3), n % 4 == 0, n < N, reads beside the sums; without Epi::vec nothing,
-// the outputs go one by one then.  A launch meets its epilogue's code cold, a miss for every line that a branch leads
-// to, so the way that calls take is kept short and straight and everything else out of it.
+// What the epilogue of four outputs (row, n .. n + 3), n < N, reads beside the sums: asked for apart from their use, so that a
+// kernel can have the loads of several on their way.  A launch meets its epilogue's code cold, a miss for every line
+// that a branch leads to, so the way that calls take is kept short and straight and everything else out of it.
 struct EpiOperands {
     f4_t bias, bias_up, residual;
 };
 template <bool kGated>
-__device__ __forceinline__ EpiOperands epi_fetch4(const Epi &e, int64_t row, int n, int expert)
+__device__ __forceinline__ EpiOperands epi_fetch_bias(const Epi &e, int n, int expert)
 {
     EpiOperands o;
     o.bias = o.bias_up = o.residual = f4_t{0.f, 0.f, 0.f, 0.f};
-    if (e.bias && e.vec) {
+    if (e.bias) {
         const int64_t b = (int64_t)expert * (kGated ? 2 * (int64_t)e.N : e.N) + n;
-        o.bias = epi_load4(e.bias, b, e.bias_f32);
-        if (kGated) o.bias_up = epi_load4(e.bias, b + e.N, e.bias_f32);
+        o.bias = epi_load4(e.bias, b, e.bias_f32, e.N - n);
+        if (kGated) o.bias_up = epi_load4(e.bias, b + e.N, e.bias_f32, e.N - n);
     }
-    if (e.residual && e.vec) o.residual = epi_load4(e.residual, row * e.N + n, e.residual_f32);
+    return o;
+}
+__device__ __forceinline__ f4_t epi_fetch_residual(const Epi &e, int64_t row, int n)
+{
+    if (!e.residual) return f4_t{0.f, 0.f, 0.f, 0.f};
+    return epi_load4(e.residual, row * e.N + n, e.residual_f32, e.N - n);
+}
+template <bool kGated>
+__device__ __forceinline__ EpiOperands epi_fetch4(const Epi &e, int64_t row, int n, int expert)
+{
+    EpiOperands o = epi_fetch_bias<kGated>(e, n, expert);
+    o.residual = epi_fetch_residual(e, row, n);
     return o;
 }
 
 // the four outputs; those past N are left out
 template <bool kGated, bool kSmall>
-__device__ __forceinline__ void epi_finish4(const Epi &e, const EpiScale &sc, const EpiOperands &o, f4_t v, f4_t u, int64_t row, int n,
-                                            int expert)
+__device__ __forceinline__ void epi_finish4(const Epi &e, const EpiScale &sc, const EpiOperands &o, f4_t v, f4_t u, int64_t row, int n)
 {
-    if (__builtin_expect(!e.vec, 0)) {
-#pragma unroll 1
-        for (int i = n; i < n + 4; i++) {   // the sums turned by one element each time: the code once
-            if (i < e.N) epi_store1<kGated>(e, sc, v[0], u[0], row, i, expert);
-            v = f4_t{v[1], v[2], v[3], v[0]};
-            u = f4_t{u[1], u[2], u[3], u[0]};
-        }
-        return;
-    }
     f4_t z = epi_act4<kSmall>(v * sc.s + o.bias, e.act);
     if (kGated) z *= u * sc.up + o.bias_up;
     z += o.residual;   // zeros if there is none
-    const int64_t i = row * e.N + n;
-    if (__builtin_expect(e.out_f32, 0)) {
-        *reinterpret_cast<f4_t *>(reinterpret_cast<float *>(e.y) + i) = z;
-    } else {
-        h4_t h;
-#pragma unroll
-        for (int k = 0; k < 4; k++) h[k] = (half_t)z[k];
-        *reinterpret_cast<h4_t *>(reinterpret_cast<half_t *>(e.y) + i) = h;
-    }
+    epi_put4(e.y, row * e.N + n, e.out_f32, e.N - n, z);
 }
 
 template <bool kGated, bool kSmall>
 __device__ __forceinline__ void epi_store4(const Epi &e, const EpiScale &sc, const f4_t &v, const f4_t &u, int64_t row, int n, int expert)
 {
     if (n >= e.N) return;
-    epi_finish4<kGated, kSmall>(e, sc, epi_fetch4<kGated>(e, row, n, expert), v, u, row, n, expert);
+    epi_finish4<kGated, kSmall>(e, sc, epi_fetch4<kGated>(e, row, n, expert), v, u, row, n);
 }
 
 // ------------------------------------------------------------------ rows by expert

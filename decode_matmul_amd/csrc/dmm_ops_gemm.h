@@ -52,15 +52,31 @@ struct GemmOpsPlace {
                     *reinterpret_cast<f4_t *>(tile + (j * 32 + l32) * kPitch + c) =
                         f4_t{acc[i][j][4 * e4], acc[i][j][4 * e4 + 1], acc[i][j][4 * e4 + 2], acc[i][j][4 * e4 + 3]};
                 }
-        __syncthreads();
-        const EpiScale sc = epi_scale(epi, expert);
-        constexpr int kPer = kOutN / 4;            // threads per row
+        // a thread has one place in the columns for all its rows: the bias comes once, the residual kAhead rows at a time
+        constexpr int kPer = kOutN / 4, kStep = 256 / kPer, kAhead = 4;
         const int c = (tid % kPer) * 4, n = n0 + c;
-        for (int r = tid / kPer; r < 32 * TM && m0 + r < m_end; r += 256 / kPer) {
-            const float *src = tile + r * kPitch + c;
-            const f4_t v = *reinterpret_cast<const f4_t *>(src);
-            const f4_t u = kGated ? *reinterpret_cast<const f4_t *>(src + kOutN) : f4_t{0.f, 0.f, 0.f, 0.f};
-            epi_store4<kGated, false>(epi, sc, v, u, m0 + r, n, expert);
+        const EpiScale sc = epi_scale(epi, expert);
+        EpiOperands ops;
+        if (n < epi.N) ops = epi_fetch_bias<kGated>(epi, n, expert);
+        __syncthreads();
+        if (n >= epi.N) return;
+        const int rows = m_end - m0 < 32 * TM ? m_end - m0 : 32 * TM;
+        for (int r0 = tid / kPer; r0 < rows; r0 += kStep * kAhead) {
+            f4_t res[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; j++)
+                res[j] = r0 + j * kStep < rows ? epi_fetch_residual(epi, m0 + r0 + j * kStep, n) : f4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int j = 0; j < kAhead && r0 + j * kStep < rows; j++) {   // (turned by one each time: the activation's code once)
+                const int r = r0 + j * kStep;
+                const float *src = tile + r * kPitch + c;
+                const f4_t v = *reinterpret_cast<const f4_t *>(src);
+                const f4_t u = kGated ? *reinterpret_cast<const f4_t *>(src + kOutN) : f4_t{0.f, 0.f, 0.f, 0.f};
+                ops.residual = res[0];
+#pragma unroll
+                for (int i = 0; i + 1 < kAhead; i++) res[i] = res[i + 1];
+                epi_finish4<kGated, false>(epi, sc, ops, v, u, m0 + r, n);
+            }
         }
     }
 };
@@ -119,19 +135,9 @@ __global__ __launch_bounds__(256) void ops_splitk_kernel(const float *__restrict
     const int64_t row = kGated ? 2 * (int64_t)epi.N : epi.N, plane = (int64_t)M * row;
     const float *src = part + m * row + n;
     f4_t v = f4_t{0.f, 0.f, 0.f, 0.f}, u = v;
-    if ((epi.N & 3) == 0) {
-        for (int z = 0; z < splits; z++) {
-            v += *reinterpret_cast<const f4_t *>(src + z * plane);
-            if (kGated) u += *reinterpret_cast<const f4_t *>(src + z * plane + epi.N);
-        }
-    } else {
-        for (int z = 0; z < splits; z++)
-#pragma unroll
-            for (int k = 0; k < 4; k++)
-                if (n + k < epi.N) {
-                    v[k] += src[z * plane + k];
-                    if (kGated) u[k] += src[z * plane + epi.N + k];
-                }
+    for (int z = 0; z < splits; z++) {
+        v += epi_load4(src + z * plane, 0, 1, epi.N - n);
+        if (kGated) u += epi_load4(src + z * plane + epi.N, 0, 1, epi.N - n);
     }
     epi_store4<kGated, false>(epi, epi_scale(epi, 0), v, u, m, n, 0);
 }

@@ -42,8 +42,6 @@ Epi make_epi(const dmm_epilogue &ep, void *y, int64_t N, const float *scales, in
     e.bias_f32 = ep.bias_type == DMM_F32;
     e.residual_f32 = ep.residual_type == DMM_F32;
     e.out_f32 = ep.out_type == DMM_F32;
-    auto four = [](const void *p, int type) { return !p || aligned(p, 4 * type_bytes(type)); };
-    e.vec = (N & 3) == 0 && four(y, ep.out_type) && four(ep.bias, ep.bias_type) && four(ep.residual, ep.residual_type);
     return e;
 }
 

@@ -154,10 +154,14 @@ __global__ __launch_bounds__(64 * kMidW) void ops_mid_kernel(OpsRowsArgs args)
             for (int t = 0; t < NT; t += kGated ? 2 : 1) {
                 if (t >= mine) break;
                 const int n = (job.it.unit + wave + (kGated ? t >> 1 : t) * W) * 16 + 4 * q;
+                if (n >= N) continue;
+                EpiOperands ops = epi_fetch_bias<kGated>(epi, n, job.it.expert);   // one for both groups of rows
 #pragma unroll
                 for (int gi = 0; gi < CG; gi++) {
                     const int m = job.it.row + gi * 16 + c16;
-                    if (m < job.it.row_end) epi_store4<kGated, true>(epi, sc, acc[t][gi], acc[kGated ? t + 1 : t][gi], m, n, job.it.expert);
+                    if (m >= job.it.row_end) continue;
+                    ops.residual = epi_fetch_residual(epi, m, n);
+                    epi_finish4<kGated, true>(epi, sc, ops, acc[t][gi], acc[kGated ? t + 1 : t][gi], m, n);
                 }
             }
         }

@@ -519,7 +519,7 @@ __device__ __forceinline__ uint32_t ops_rows_body(const OpsRowsArgs &args, uint3
                         }
                         if (jc == 15 && cell_live(cell)) {
                             if (c0 > 0) ops0 = epi_fetch4<kGated>(epi, cell_row(cell), cell_col(cell), it.expert);
-                            epi_finish4<kGated, true>(epi, sc, ops0, v, up, cell_row(cell), cell_col(cell), it.expert);
+                            epi_finish4<kGated, true>(epi, sc, ops0, v, up, cell_row(cell), cell_col(cell));
                         }
                     }
                 } else {
