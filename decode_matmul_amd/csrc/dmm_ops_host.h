@@ -219,19 +219,43 @@ int run_ops_rows(const void *x, const void *codes, const void *grid, const Group
     return launch_ops_rows<8, 8, 1, kGated>(x, codes, grid, g, e, K, s);
 }
 
-// More than 32 rows, dense: the few-rows kernel (32 rows per segment) or split K / the matrix-matrix kernel.  The first costs
-// about 7 us, K * 0.34 ns per 16-row tile of the busiest workgroup and 3.5 us for every eight of them after the first;
-// the split what passes_beat_splitk says, 14 us + 0.085 per row + 0.3 per MB of codes (graph launches, us, few rows / split:
-// 4096 x 4096 M = 64 11.6 / 20.8, 256 20.0 / 27.0, 400 33.6 / 31.2; 8192 x 8192 M = 128 31.2 / 32.4, 200 54.4 / 42.6; 4096 x 11008 M = 128
-// 26.4 / 29.8; 2 x 11008 x 4096 M = 64 30.2 / 26.2).
-bool ops_rows_beat_split(int64_t M, int64_t N, int64_t K, bool gated, int cus)
+// Estimates, in us, for segments of 32 rows (`segs` of them), N columns of y and K:
+// the kernel for tens of rows: 5 and, per 256 k, by the tiles that a wave has on average (0.25 tiles 0.7, 0.9 tiles 0.9, 2.4 tiles
+// 1.6 to 1.8, 4.4 tiles 3.0, 9 tiles 6.6);
+inline double ops_mid_cost(double segs, int64_t N, int64_t K, bool gated, int cus)
 {
-    if (M <= 32) return true;
-    if (M > 512) return false;
-    const int64_t units = (M + 31) / 32 * ((N + 15) / 16), tiles = (units + cus - 1) / cus * (gated ? 2 : 1);
-    const double rows = 7.0 + (double)tiles * (double)K * 0.34e-3 + 3.5 * (double)((tiles - 1) / 8);
-    const double split = 14.0 + 0.085 * (double)M + 0.3e-6 * (double)(gated ? 2 * N : N) * (double)(K >> 2) * (256.0 / cus);
-    return rows * 1.05 < split;
+    const double f = segs * (double)((N + 15) / 16) / (8.0 * cus);
+    return 5.0 + std::max(0.6, std::max(0.2 + 0.65 * f, 0.75 * f - 0.3)) * (gated ? 2.0 : 1.0) * (double)((K + 255) / 256);
+}
+// the matrix-matrix kernel: 15 and K * 12 ns per round of blocks (`tiles` of 128 rows).
+inline double ops_gemm_cost(double tiles, int64_t N, int64_t K, bool gated, int cus)
+{
+    const double blocks = tiles * (double)(((gated ? 2 * N : N) + 255) / 256), rounds = (double)(int64_t)(blocks / cus + 0.999);
+    return rounds * (15.0 + (double)K * 12e-3);
+}
+
+// Dense calls of more than 32 rows: the few-rows kernel (32 rows per segment), the one for tens of rows, or split K / the
+// matrix-matrix kernel (kOpsGemm stands for both).  The first costs about 7 us, K * 0.34 ns (0.5 past 512 rows, where a
+// workgroup meets many segments) per 16-row tile of the busiest workgroup and 3.5 us for every eight of them after the first; the
+// split what passes_beat_splitk says up to 512 rows, 14 us + 0.085 per row + 0.3 per MB of codes, and 16 us and 1 PF/s past them
+// (graph launches, us, few rows / tens / split: 4096 x 4096 M = 100 12.9 / 16.6 / 25.0, 400 31.9 / 27.5 / 31.4; 4096 x 11008 M = 200 36.5 / 44.1 / 34.8;
+// 2 x 137 x 11776 M = 528 24.5 / 51.3 / 49.3; 4096 x 512 M = 800 33.8 / 13.1 / 23.9; 1024 x 1024 M = 1024 12.1 / 9.2 / 22.3; 2 x 640 x
+// 768 M = 1500 20.9 / 10.2 / 23.7; 104 x 320 M = 2957 8.9 / 6.5 / 22.2; 256 x 4096 M = 4096 26.6 / 23.7 / 27.8; 1024 x 4096 M = 2048 44.3 /
+// 31.4 / 33.5; 2 x 11008 x 4096 M = 400 137 / 100 / 110, M = 600 198 / 154 / 116).
+inline OpsKernel ops_dense_choice(int64_t M, int64_t N, int64_t K, bool gated, int cus)
+{
+    if (M <= 32) return kOpsRows;
+    const int64_t segs = (M + 31) / 32, units = segs * ((N + 15) / 16), tiles = (units + cus - 1) / cus * (gated ? 2 : 1);
+    const double rows = 7.0 + (double)tiles * (double)K * (M > 512 ? 0.5e-3 : 0.34e-3) + 3.5 * (double)((tiles - 1) / 8);
+    const double mid = ops_mid_cost((double)segs, N, K, gated, cus);
+    const double n2 = gated ? 2.0 * (double)N : (double)N;
+    const double blocks = (double)((M + 127) / 128) * (double)(((int64_t)n2 + 255) / 256);
+    double large;
+    if (M > 512) large = std::min(16.0 + 2e-9 * (double)M * n2 * (double)K * (256.0 / cus), ops_gemm_cost((double)((M + 127) / 128), N, K, gated, cus));
+    else if (2 * blocks > cus) large = (double)(int64_t)(blocks / cus + 0.999) * (12.0 + (double)K * 10e-3);   // enough blocks: no split
+    else large = 14.0 + 0.085 * (double)M + 0.3e-6 * n2 * (double)(K >> 2) * (256.0 / cus);
+    if (std::min(rows, mid) >= large) return kOpsGemm;
+    return rows <= mid ? kOpsRows : kOpsMid;
 }
 
 template <bool kGated>
@@ -261,17 +285,22 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     if (rows_ok && force == kOpsRows) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
     if (mid_ok && force == kOpsMid) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
     if (g.offsets) {
-        // Up to eight rows per expert the few-rows kernel, up to 160 the one for tens of rows where every wave has a unit
+        // Up to eight rows per expert the few-rows kernel, then the one for tens of rows where every wave has a unit, or the
+        // matrix-matrix kernel, by their estimates; half a segment and half a tile of every expert are not full
         // (graph launches, us, few rows / tens / matrix-matrix, rows per expert: 2 x 11008 x 4096, 8 experts 4: 56 / 62 / 88, 8: 75 / 68 /
         // 90, 31: 127 / 92 / 181, 64: 224 / 165 / 221, 128: - / 288 / 367, 256: - / 528 / 533; 4096 x 11008, 16 experts 4: 50 / 63 / 74,
         // 8: 74 / 73 / 141, 31: 114 / 100 / 147, 128: - / 288 / 292, 256: - / 533 / 455; 2 x 1408 x 2048, 64 experts 4: 33 / 37 / 51, 8: 47 /
         // 46 / 66, 31: 93 / 65 / 99, 128: - / 159 / 196, 256: - / 294 / 274; but 4096 x 4096, 8 experts, 8 units per workgroup, 12: 20 / 24)
         const int64_t avg = g.R / g.E, units = (int64_t)g.E * ((avg + 31) / 32) * ((e.N + 15) / 16);
         if (force < 0 && rows_ok && (avg < 8 || (avg <= 64 && units <= 8LL * cus))) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
-        if (force < 0 && mid_ok && avg < 160) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
+        if (force < 0 && mid_ok && ops_mid_cost((double)g.R / 32 + 0.5 * g.E, e.N, K, kGated, cus) <=
+                                       ops_gemm_cost((double)g.R / 128 + 0.5 * g.E, e.N, K, kGated, cus))
+            return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
         return run_ops_gemm<kGated>(x, codes, grid, g, e, K, s);
     }
-    if (force < 0 && rows_ok && ops_rows_beat_split(g.R, e.N, K, kGated, cus)) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    const OpsKernel choice = force < 0 ? ops_dense_choice(g.R, e.N, K, kGated, cus) : kOpsGemm;
+    if (choice == kOpsRows && rows_ok) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
+    if (choice == kOpsMid && mid_ok) return launch_ops_mid<kGated>(x, codes, grid, g, e, K, s);
     if (force != kOpsGemm && workspace && workspace_bytes > 0 && g.R >= kSplitKMinM && (K & 63) == 0 && gemm_reg_ok(g.R, rows, K)) {
         const int splits = splitk_plan(g.R, rows, K, workspace_bytes, cus);
         if (splits >= 2) {
@@ -297,7 +326,7 @@ int64_t ops_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated)
 {
     const int64_t rows = gated ? 2 * N : N;
     if (M < kSplitKMinM || N < 1 || K < 64 || (K & 63) || M > 65535LL * 128 || !gemm_reg_ok(M, rows, K)) return 0;
-    if (ops_rows_beat_split(M, N, K, gated, cu_count_or_default()) && g_ops_kernel.load(std::memory_order_relaxed) != kOpsSplit) return 0;
+    if (ops_dense_choice(M, N, K, gated, cu_count_or_default()) != kOpsGemm && g_ops_kernel.load(std::memory_order_relaxed) != kOpsSplit) return 0;
     const int splits = splitk_plan(M, rows, K, INT64_MAX, cu_count_or_default());
     return splits >= 2 ? (int64_t)splits * M * rows * 4 : 0;
 }
