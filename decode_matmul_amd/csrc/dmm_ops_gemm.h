@@ -11,10 +11,10 @@
 //     factors of its outputs in the same elements of acc[0] and acc[1].
 //   * The sums go through the LDS (the tables and x are not needed any more) as a [row of y][column] fp32 tile with a
 //     pitch of 260 floats - 16 lanes of the 16-byte writes, one row each, meet 16 different bank groups - and come
-//     back row by row: stores and the reads of bias and residual cover whole lines (512 bytes of a row per wave
+//     back row by row: stores and the reads of the residual cover whole lines (512 bytes of a row per wave
 //     and load), and the activation's code exists once, in a loop, not once per accumulator element.
 // What bounds it: the matrix unit is busy for half of the cycles, the rest is what one wave per SIMD issues beside it, as in the
-// plain kernel.  Gate and up of 4096 -> 11008, 2048 rows 390 us (946 TF/s); the same by 8 experts, 4096 rows 858 us (861 TF/s; every
+// plain kernel.  Gate and up of 4096 -> 11008, 2048 rows 380 us (972 TF/s); the same by 8 experts, 4096 rows 863 us (856 TF/s; every
 // expert ends in a tile that is not full).
 template <bool kGated>
 struct GemmOpsPlace {

@@ -17,7 +17,7 @@
 // What bounds it: decoding once per 32 rows.  Two waves per SIMD share its issue: vector ALU 42 %, LDS 38 %, matrix unit 26 % of the
 // cycles; gathers a word further ahead (also across tiles) change nothing, and 64 rows per segment (a decode for
 // four groups, x a step of 256 k at a time, no registers left to read it ahead) took 20 % longer at 31 rows per expert and as
-// long at 128.  2 x 1408 x 2048, 64 experts, 1998 rows 63.3 us (364 TF/s); 2 x 11008 x 4096, 8 experts, 512 rows 165 us (560 TF/s).
+// long at 128.  2 x 1408 x 2048, 64 experts, 1998 rows 60.3 us (382 TF/s); 2 x 11008 x 4096, 8 experts, 512 rows 165 us (560 TF/s).
 // LDS map: tables [0, 96K), x buffers [96K, 160K).
 constexpr int kMidW = 8, kMidRows = 32, kMidChunk = 512, kMidXBuf = kMidRows * kMidChunk * 2;
 constexpr int kMidBytes = kSTablesBytes + 2 * kMidXBuf;
