@@ -108,6 +108,14 @@ inline bool ops_jobs_fit(const Groups &g, int64_t sr, int64_t N)
     return (g.offsets ? (int64_t)g.E : 1) * (((int64_t)g.R + sr - 1) / sr) * ((N + 15) / 16) < (1LL << 31);
 }
 
+// A job that 8-bit operands cannot do is done again in 16 bits, by number up to the 32nd of a workgroup's; the ones behind it
+// share a bit, so that some are stored twice.  That changes nothing, except where the residual is the output itself: it
+// would be added twice.  Whether no workgroup has more jobs than numbers (a job is one unit or more).
+inline bool ops_redo_by_number(const Groups &g, int64_t N, int64_t cus)
+{
+    return ops_segments(g, 2) * ((N + 15) / 16) <= 32 * cus;
+}
+
 template <int XI, int W, int CG, bool kGated>
 int launch_ops_rows(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
 {
@@ -273,10 +281,8 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
         return launch_ops_stream(x, codes, grid, g, e, K, s);
     if (one_row && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled()) return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
     // 8-bit operands, two rows per segment: one or two rows of a dense call, and by expert where few experts have a row and
-    // the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7 us, 16-bit 14.4; 2 rows 18.9 / 21.1; but 4 rows 24.7 / 20.6).  A
-    // job they cannot do is done again in 16 bits, by number up to the 31st; behind it jobs may be stored twice,
-    // which a residual that is the output itself would not survive.
-    const bool rows8_ok = ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (!e.residual || (int64_t)e.N <= 24LL * 16 * 2 * cus);
+    // the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7 us, 16-bit 14.4; 2 rows 18.9 / 21.1; but 4 rows 24.7 / 20.6).
+    const bool rows8_ok = ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (e.residual != e.y || ops_redo_by_number(g, e.N, cus));
     const bool rows8_pays = g.offsets ? (g.R <= 2 || 4 * (int64_t)g.R <= g.E) && K >= 4096 &&
                                             std::min<int64_t>(g.R, g.E) * rows * (K >> 2) >= (20LL << 20)
                                       : g.R <= 2;
