@@ -80,6 +80,7 @@ const char *dmm_status_string(int status)
             return "the split-K partial sums of this shape exceed the library's 16 MiB scratch buffer: use "
                    "dmm_decode_matmul_ws_f16 with a workspace of dmm_workspace_bytes, or dmm_decode_matmul_f16";
         case DMM_ERR_HOST_MEMORY: return "host memory for a decoded row could not be allocated";
+        case DMM_ERR_OVERLAP: return "the residual shares memory with the output without being the output itself";
         default: break;
     }
     if (status > 0) return hipGetErrorString((hipError_t)status);

@@ -7,6 +7,15 @@ inline uintptr_t type_bytes(int t) { return t == DMM_F32 ? 4 : 2; }
 // rows of x and of y in one call: row numbers of a tile that begins at the last row stay below 2^31
 constexpr int64_t kOpsMaxRows = 1 << 30;
 
+// Residual and output, n elements each: the same memory, element for element, or none in common.  (A half residual and a
+// float output at one address would overwrite elements that are still to be read.)
+inline bool residual_ok(const void *residual, int residual_type, const void *y, int out_type, int64_t n)
+{
+    if (!residual || (residual == y && residual_type == out_type)) return true;
+    const uintptr_t r = reinterpret_cast<uintptr_t>(residual), o = reinterpret_cast<uintptr_t>(y);
+    return r + (uintptr_t)n * type_bytes(residual_type) <= o || o + (uintptr_t)n * type_bytes(out_type) <= r;
+}
+
 // what both products ask of their arguments: T rows of x, R rows of y, E matrices
 int check_ops(const void *x, int64_t T, const void *codes, const void *grid, const dmm_epilogue *ep, const void *y, int64_t R,
               int64_t E, int64_t N, int64_t K)
@@ -24,6 +33,7 @@ int check_ops(const void *x, int64_t T, const void *codes, const void *grid, con
         (ep->residual && !aligned(ep->residual, type_bytes(ep->residual_type))))
         return DMM_ERR_MISALIGNED;
     if (T > kOpsMaxRows || R > kOpsMaxRows || E > 65535 || N > INT32_MAX / 2 || K > INT32_MAX) return DMM_ERR_TOO_LARGE;
+    if (!residual_ok(ep->residual, ep->residual_type, y, ep->out_type, R * N)) return DMM_ERR_OVERLAP;
     return DMM_OK;
 }
 
@@ -513,5 +523,6 @@ int check_combine(const void *y, int y_type, const void *slots, const void *weig
         (residual && !aligned(residual, type_bytes(residual_type))))
         return DMM_ERR_MISALIGNED;
     if (R > INT32_MAX || T > INT32_MAX || k > INT32_MAX || N > INT32_MAX - 4096) return DMM_ERR_TOO_LARGE;
+    if (!residual_ok(residual, residual_type, out, out_type, T * N)) return DMM_ERR_OVERLAP;
     return DMM_OK;
 }

@@ -53,7 +53,9 @@ enum {
                                    static LDS); no kernel was launched                  */
     DMM_ERR_SCRATCH_TOO_SMALL = -8, /* dmm_decode_matmul_noalloc_f16: the shape's partial
                                    sums exceed the library's scratch buffer             */
-    DMM_ERR_HOST_MEMORY = -9    /* dmm_decode_matmul_host_f16: malloc of a row failed   */
+    DMM_ERR_HOST_MEMORY = -9,   /* dmm_decode_matmul_host_f16: malloc of a row failed   */
+    DMM_ERR_OVERLAP = -10       /* a residual shares memory with the output without being
+                                   the output itself, element for element               */
 };
 
 /* Library version, (major << 16) | minor. */
@@ -293,7 +295,8 @@ enum { DMM_ACT_NONE = 0, DMM_ACT_RELU = 1, DMM_ACT_SILU = 2, DMM_ACT_GELU = 3, D
  *   y = act(z[n]) * z[N + n]                                      gated != 0: W has 2 N rows, gate then up
  *   y += residual
  * Types are DMM_F16 or DMM_F32; a NULL bias or residual is left out and its type not looked at.  y may be the residual
- * itself and shares memory with no other input. */
+ * itself (the same address and the same type; any other overlap of the two is refused with DMM_ERR_OVERLAP) and shares
+ * memory with no other input. */
 typedef struct dmm_epilogue {
     const void *bias;        /* [N], gated [2 N] (grouped: one such row per expert)       */
     const void *residual;    /* [M, N]; may be y itself.  dmm_decode_matmul_grouped: NULL  */
@@ -357,8 +360,8 @@ int dmm_route_experts(const void *logits, int logits_type, int64_t T, int64_t E,
 
 /* The weighted sum of the experts' rows: out[t] = residual[t] + sum over j, in order, of weights[t,j] * y[slots[t,j]], in fp32
  * with one rounding; y [R,N] and out [T,N] half or float, weights float [T,k], slots int32 [T,k].  A slot outside
- * 0 .. R - 1 adds nothing.  residual [T,N] half or float, or NULL; it may be out itself.  out shares memory with no
- * other input. */
+ * 0 .. R - 1 adds nothing.  residual [T,N] half or float, or NULL; it may be out itself (the same address and the same
+ * type; any other overlap of the two is refused with DMM_ERR_OVERLAP).  out shares memory with no other input. */
 int dmm_combine_experts(const void *y, int y_type, const void *slots, const void *weights, const void *residual,
                         int residual_type, void *out, int out_type, int64_t R, int64_t T, int64_t k, int64_t N,
                         void *stream);

@@ -1,0 +1,46 @@
+"""Calls of the operators around the product that the library refuses, or has to take, before any GPU call."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import decode_matmul_amd as dmm
+from decode_matmul_amd import capi
+from ops_util import assert_within, combine64, decode64, fused_inputs, grouped64, grouped_inputs, product64
+
+F16, F32 = torch.float16, torch.float32
+OVERLAP = -10
+
+
+# ----------------------------------------------------------------- a residual that overlaps the output
+def test_residual_that_overlaps_the_output_is_refused():
+    lib = capi.lib()
+    buf = (ctypes.c_uint16 * 8192)()
+    p = ctypes.addressof(buf)
+    M, N, K = 4, 8, 16
+    assert b"residual" in lib.dmm_status_string(OVERLAP)
+
+    def fused(fn, residual, residual_type, y, out_type):
+        e = capi.Epilogue(residual=residual, residual_type=residual_type, out_type=out_type, scale=1.0, scale_up=1.0)
+        tail = (None, 0, None) if fn is lib.dmm_decode_matmul_fused else ()
+        return fn(p, p + 1024, p + 2048, ctypes.byref(e), y, M, N, K, *tail)
+
+    def combine(fn, residual, residual_type, out, out_type):
+        tail = (None,) if fn is lib.dmm_combine_experts else ()
+        return fn(p, 0, p + 1024, p + 2048, residual, residual_type, out, out_type, 4, M, 2, N, *tail)
+
+    y = p + 8192
+    for call, fns in ((fused, (lib.dmm_decode_matmul_fused, lib.dmm_decode_matmul_fused_host)),
+                      (combine, (lib.dmm_combine_experts, lib.dmm_combine_experts_host))):
+        for fn in fns:
+            assert call(fn, y, 0, y, 1) == OVERLAP              # half elements under float ones
+            assert call(fn, y, 1, y, 0) == OVERLAP
+            assert call(fn, y + 2, 0, y, 0) == OVERLAP          # one element further on
+            assert call(fn, y - 2 * M * N + 2, 0, y, 0) == OVERLAP
+            assert call(fn, y + 4 * M * N - 2, 0, y, 1) == OVERLAP
+        host = fns[1]
+        assert call(host, y, 0, y, 0) == 0                      # the output itself
+        assert call(host, y, 1, y, 1) == 0
+        assert call(host, y + 2 * M * N, 0, y, 0) == 0          # side by side
+        assert call(host, y - 2 * M * N, 0, y, 1) == 0
