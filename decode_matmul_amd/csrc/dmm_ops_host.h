@@ -290,12 +290,19 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     if (!kGated && one_row && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cus && ops_stream_lds(K) <= kLdsMax)
         return launch_ops_stream(x, codes, grid, g, e, K, s);
     if (one_row && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled()) return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
-    // 8-bit operands, two rows per segment: one or two rows of a dense call, and by expert where few experts have a row and
-    // the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7 us, 16-bit 14.4; 2 rows 18.9 / 21.1; but 4 rows 24.7 / 20.6).
+    // 8-bit operands, two rows per segment.  One or two rows of a dense call: from three tiles per compute unit on, or two on a
+    // long K, and not on a short one; elsewhere the 16-bit kernel is as fast or faster and its sums are exact products' (graph
+    // launches, us, 8-bit / 16-bit, two rows: 1024 -> 4096 4.76 / 3.93, 4096 -> 4096 5.10 / 4.72, 11008 -> 4096 7.10 / 6.73, 28672 -> 4096
+    // 13.5 / 12.3, 4096 -> 8192 5.52 / 5.36, 8192 -> 8192 7.05 / 7.10, 4096 -> 2 x 2048 5.58 / 5.40, 1024 -> 32000 7.4 / 6.4, 2048 -> 22016 7.1 /
+    // 6.5, 512 -> 128000 21.9 / 19.2; but 2560 -> 16384 6.26 / 6.44, 4096 -> 11008 6.20 / 6.29, 4096 -> 22016 8.46 / 9.24, 8192 -> 28672 14.6 /
+    // 16.8, 12288 -> 8192 9.4 / 9.9, 28672 -> 8192 16.4 / 17.2, 4096 -> 2 x 11008 8.72 / 9.35, 8192 -> 2 x 28672 30.5 / 35.5).  By
+    // expert where few experts have a row and the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7, 16-bit 14.4; 2 rows
+    // 18.9 / 21.1; but 4 rows 24.7 / 20.6).
     const bool rows8_ok = ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (e.residual != e.y || ops_redo_by_number(g, e.N, cus));
+    const int64_t share = ops_share(e.N, kGated);
     const bool rows8_pays = g.offsets ? (g.R <= 2 || 4 * (int64_t)g.R <= g.E) && K >= 4096 &&
                                             std::min<int64_t>(g.R, g.E) * rows * (K >> 2) >= (20LL << 20)
-                                      : g.R <= 2;
+                                      : g.R <= 2 && K > 2048 && (share >= 3 || (share == 2 && K >= 12288));
     if (rows8_ok && (force == kOpsRows8 || (force < 0 && rows8_pays && gemv_q8_enabled())))
         return run_ops_rows8<kGated>(x, codes, grid, g, e, K, s);
     if (rows_ok && force == kOpsRows) return run_ops_rows<kGated>(x, codes, grid, g, e, K, s);
