@@ -336,7 +336,10 @@ int dmm_decode_matmul_grouped(const void *x, int64_t T, const void *rows, const 
  * 0 the catch-all, 1 the kernel for few rows, 2 the matrix-matrix kernel, 3 the same with split K (where a
  * workspace is given), 4 the kernel for few rows on 8-bit operands (half outputs), 5 the kernel for tens of rows;
  * -1: the library's own choice.  A forced kernel that cannot take a call leaves it to one that
- * can.  Returns the previous value (>= -1), or DMM_ERR_BAD_SHAPE.  Results differ by the order of the sums only. */
+ * can.  Returns the previous value (>= -1), or DMM_ERR_BAD_SHAPE.  Results of 0 to 3 and 5 are sums of exact products and
+ * differ by the order of the sums only.  4, and the library's choice for one and two rows, has the arithmetic of
+ * dmm_gemv_8bit_f16: the shift's products go through means of eight x with 22 bits, the matrix unit cuts
+ * the products it adds at a time at the last bit of the largest. */
 int dmm_set_ops_kernel(int kernel);
 
 /* The choice of experts: for every row of logits [T,E] (half, bfloat16 or float) the k largest, largest first, equal ones

@@ -1,5 +1,4 @@
 """The operators around the product as a user gets them: the library's own choice, 8-bit operands in their default position."""
-import ctypes
 import math
 
 import pytest
@@ -8,7 +7,8 @@ import torch
 import decode_matmul_amd as dmm
 from decode_matmul_amd import capi
 from gpu_util import DEV
-from ops_util import (ACTS, assert_within, check_routing, combine64, decode64, fused_inputs, grouped64, grouped_inputs, product64, weights)
+from ops_terms import Case, cancelling, grouped8
+from ops_util import assert_within, check_routing, combine64, decode64, fused_inputs, product64, weights
 
 pytestmark = pytest.mark.gpu
 F16, F32 = torch.float16, torch.float32
@@ -36,3 +36,202 @@ def test_few_tiles_keep_16_bit_operands(M, N, K, gated):
     y = dmm.decode_matmul_fused(*args, 1 / math.sqrt(K), gated=gated)
     capi.lib().dmm_set_gemv_8bit(0)
     assert torch.equal(y, dmm.decode_matmul_fused(*args, 1 / math.sqrt(K), gated=gated))
+
+
+# ----------------------------------------------------------------- every term of x and both halves of the means
+def check_cancelled(y, left, tol):
+    """y = what a bias leaves of the sums: left up to tol, in fp32 (two roundings of the sum and the bias are in tol), rounded to half."""
+    bound = tol + 2.0 ** -11 * (left.abs() + tol) + 2.0 ** -25
+    err = (y.detach().cpu().double() - left).abs()
+    assert torch.all(err <= bound), "%d of %d outside, worst %.3g of the bound" % (int((err > bound).sum()), err.numel(), float((err / bound).max()))
+
+
+def check_terms(M, N, K, gated, first=0, count=None):
+    if not gated:
+        c = Case(M, N, K, M + N + K + first, first, count)
+        b, left = cancelling(c)
+        y = dmm.decode_matmul_fused(*dev(c.x, c.codes, c.grid), 1.0, bias=b.to(DEV))
+        assert y.dtype == F16
+        check_cancelled(y, left.expand(M, N), c.tol())
+        return
+    c = Case(M, 2 * N, K, M + N + K + first, first, count)
+    for who in (0, 1):      # one factor's sums cancel, the other factor is 64
+        keep = torch.full((2 * N,), 64.0, dtype=torch.float64)
+        keep[who * N:(who + 1) * N] = 0
+        b, left = cancelling(c, keep)
+        y = dmm.decode_matmul_fused(*dev(c.x, c.codes, c.grid), 1.0, bias=b.to(DEV), gated=True)
+        gate, up = left[:N], left[N:]
+        t = c.tol()
+        check_cancelled(y, (gate * up).expand(M, N), (t * (gate.abs() + up.abs() + t) + 2.0 ** -24 * (gate * up).abs()).expand(M, N))
+
+
+# tiles per compute unit (256 of them): gemv_q8d's body with 2, 4, 6 and 8 tiles, plain and in pairs, tails of all kinds
+@pytest.mark.parametrize("N,gated", [(4095, False), (8192, False), (12288, False), (16383, False), (16386, False), (24575, False),
+                                     (24580, False), (32766, False), (2049, True), (4096, True), (8189, True), (11008, True),
+                                     (12285, True), (16382, True)])
+@pytest.mark.parametrize("K,first,count", [(256, 0, None), (2048, 0, None), (8192, 0, 32), (8192, 500, 32), (8192, 992, 32)])
+def test_one_row_sees_every_term(N, K, first, count, gated):
+    check_terms(1, N, K, gated, first, count)
+
+
+# the jobs' kernel: one job and many, one row and two, K that is not whole steps
+@pytest.mark.parametrize("M,N,gated", [(1, 40004, False), (1, 20001, True), (2, 14000, False), (2, 33001, False), (2, 8197, True), (2, 20001, True)])
+@pytest.mark.parametrize("K,first,count", [(2304, 0, 32), (4352, 400, 32), (4352, 512, 32), (2064, 256, 2), (2064, 240, 18), (8192, 992, 32)])
+def test_one_and_two_rows_in_jobs_see_every_term(M, N, gated, K, first, count):
+    check_terms(M, N, K, gated, first, count)
+
+
+# forced where the choice would not take it: short K, few tiles, many segments
+@pytest.mark.parametrize("M,N,gated", [(1, 17, False), (2, 16, True), (1, 5000, False), (2, 9001, True)])
+@pytest.mark.parametrize("K", [16, 64, 240, 256])
+def test_short_k_in_jobs_sees_every_term(M, N, gated, K):
+    capi.lib().dmm_set_ops_kernel(4)
+    check_terms(M, N, K, gated)
+
+
+def grouped_terms(counts, N, K, seed, first=0, count=None):
+    """Every expert its own case; up to two rows each, as tokens in an order of their own; the biases cancel all sums."""
+    cases = [Case(max(n, 1), N, K, seed + e, first, count) for e, n in enumerate(counts)]
+    T = sum(counts)
+    order = torch.randperm(T, generator=torch.Generator().manual_seed(seed))
+    x = torch.zeros(T, K, dtype=F16)
+    x[order] = torch.cat([c.x[:n] for c, n in zip(cases, counts) if n > 0])
+    offsets = torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=torch.int32)
+    b, left = zip(*(cancelling(c) for c in cases))
+    want = torch.cat([v.expand(n, -1) for v, n in zip(left, counts)])
+    tol = torch.cat([torch.full((n, N), c.tol(), dtype=torch.float64) for c, n in zip(cases, counts)])
+    return x, torch.stack([c.codes for c in cases]), cases[0].grid, offsets, order.int(), torch.stack(b), want, tol
+
+
+# by expert, by the library's own rule: up to two rows in all, and a quarter as many rows as experts, on 20 MB of codes and more
+@pytest.mark.parametrize("counts,N,K,first,count", [((0, 1, 0, 1), 10300, 4096, 0, 32), ((0, 0, 2), 22000, 4096, 300, 32),
+                                                    ((0, 1), 21001, 4352, 512, 32), ((0, 2, 0, 0, 0, 0, 1, 0) + (0,) * 5 + (1, 0, 0), 5500, 4096, 480, 32)])
+def test_grouped_sees_every_term(counts, N, K, first, count):
+    x, codes, grid, offsets, rows, b, want, tol = grouped_terms(counts, N, K, 7, first, count)
+    args = dev(x, codes, grid)
+    kw = dict(rows=rows.to(DEV), bias=b.to(DEV))
+    y = dmm.decode_matmul_grouped(*args, 1.0, offsets.to(DEV), **kw)
+    check_cancelled(y, want, tol)
+
+
+@pytest.mark.parametrize("counts,N,K", [((1, 2, 0, 2, 1, 1), 9001, 256), ((2,) * 70, 200, 256), ((0,) * 66 + (2, 0, 1), 777, 256), ((1, 2), 40, 112)])
+def test_grouped_many_jobs_see_every_term(counts, N, K):
+    capi.lib().dmm_set_ops_kernel(4)
+    x, codes, grid, offsets, rows, b, want, tol = grouped_terms(counts, N, K, 11)
+    y = dmm.decode_matmul_grouped(*dev(x, codes, grid), 1.0, offsets.to(DEV), rows=rows.to(DEV), bias=b.to(DEV))
+    check_cancelled(y, want, tol)
+
+
+@pytest.mark.parametrize("N,gated", [(4095, False), (8192, False), (16383, False), (24575, False), (32766, False), (2049, True), (8189, True),
+                                     (11008, True), (16382, True)])
+@pytest.mark.parametrize("what", ["grid", "infinity", "nan"])
+def test_one_row_that_8_bit_operands_cannot_do(N, gated, what):
+    """The batch-1 body hands the launch over to 16 bits: the sums of exact products, and an infinity only where it belongs."""
+    K = 512
+    x, codes, grid, b, r = fused_inputs(1, N, K, gated, F16, F16, N, fp8=what != "grid")
+    if what != "grid":
+        x[0, 300] = math.inf if what == "infinity" else math.nan
+    y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.05, bias=b.to(DEV), gated=gated, residual=r.to(DEV))
+    want, tol = product64(x.double(), decode64(codes, grid), (0.05, 0.05), b, gated, "none", r, F16)
+    if what == "grid":
+        assert_within(y, want, tol)
+        return
+    got = y.cpu().double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    live = ~torch.isnan(want)
+    assert torch.equal(got[live], want[live])        # infinities of the right sign
+
+
+# ----------------------------------------------------------------- together, as a layer uses them
+def layer_weights(E, H, N, seed):
+    gen = torch.Generator().manual_seed(seed)
+    up, grid = weights(gen, E, 2 * N, H // 8)
+    down, _ = weights(gen, E, H, N // 8)
+    dense, _ = weights(gen, 2 * N, H // 8)
+    back, _ = weights(gen, H, N // 8)
+    return up, down, dense, back, grid
+
+
+def layer(x, logits, up, down, dense, back, grid, H, N, k=2):
+    """Routed experts and a shared dense MLP whose result is the residual of their sum."""
+    h = dmm.decode_matmul_fused(x, dense, grid, 1 / math.sqrt(H), gated=True, activation="silu")
+    shared = dmm.decode_matmul_fused(h, back, grid, 1 / math.sqrt(N), residual=x)
+    r = dmm.route_experts(logits, k)
+    g = dmm.decode_matmul_grouped(x, up, grid, 1 / math.sqrt(H), r.offsets, rows=r.rows, activation="silu", gated=True)
+    o = dmm.decode_matmul_grouped(g, down, grid, 1 / math.sqrt(N), r.offsets)
+    return r, h, shared, g, o, dmm.combine_experts(o, r.slots, r.weights, residual=shared)
+
+
+@pytest.mark.parametrize("T", [1, 2, 5])
+def test_a_decode_step_through_a_layer(T):
+    """4096 -> 2 x 5376, two of four experts and a shared MLP: one token takes every kernel on 8-bit operands."""
+    H, N, E, k = 4096, 5376, 4, 2
+    up, down, dense, back, grid = layer_weights(E, H, N, T)
+    gen = torch.Generator().manual_seed(T + 100)
+    x, logits = torch.randn(T, H, generator=gen).half(), torch.randn(T, E, generator=gen)
+    r, h, shared, g, o, y = layer(*dev(x, logits, up, down, dense, back, grid), H, N)
+    check_routing(r, logits, k, "softmax", True)
+    all_rows, one = torch.arange(T, dtype=torch.int32), torch.tensor([0, T])
+    assert_within(h, *grouped8(x, dense[None], grid, 1 / math.sqrt(H), one, all_rows, True, "silu", F16, N))
+    want, tol = grouped8(h.cpu(), back[None], grid, 1 / math.sqrt(N), one, all_rows, False, "none", F16, H)
+    want = want + x.double()
+    assert_within(shared, want, tol + 2.0 ** -11 * want.abs())
+    assert_within(g, *grouped8(x, up, grid, 1 / math.sqrt(H), r.offsets.cpu(), r.rows.cpu(), True, "silu", F16, N))
+    assert_within(o, *grouped8(g.cpu(), down, grid, 1 / math.sqrt(N), r.offsets.cpu(), torch.arange(T * k, dtype=torch.int32), False, "none", F16, H))
+    assert_within(y, *combine64(o.cpu(), r.slots.cpu(), r.weights.cpu(), shared.cpu(), F16))
+
+
+@pytest.mark.parametrize("T", [1, 2, 24])
+def test_captured_decode_step_follows_its_inputs(T):
+    """Replays with other tokens, other choices, an infinity, and a grid that does not fit 8 bits give what eager calls give."""
+    H, N, E = 4096, 5376, 4
+    up, down, dense, back, grid = dev(*layer_weights(E, H, N, 3))
+    other = weights(torch.Generator().manual_seed(5), 1, 1, fp8=False)[1].to(DEV)
+    x, logits, g = torch.empty(T, H, dtype=F16, device=DEV), torch.empty(T, E, device=DEV), torch.empty_like(grid)
+
+    def fill(seed):
+        gen = torch.Generator().manual_seed(seed)
+        x.copy_(torch.randn(T, H, generator=gen))
+        if seed == 3:
+            x[T - 1, 77] = math.inf
+        logits.copy_(torch.randn(T, E, generator=gen))
+        g.copy_(other if seed == 4 else grid)
+
+    def step():
+        return layer(x, logits, up, down, dense, back, g, H, N)[-1]
+
+    capi.check("dmm_init", capi.lib().dmm_init(-1))
+    fill(0)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            y = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for seed in (1, 2, 3, 4, 5):
+        fill(seed)
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y.view(torch.int16), want.view(torch.int16)), seed
+        assert torch.isfinite(want).all() == (seed != 3)
+
+
+@pytest.mark.parametrize("M,N,K,gated", [(1, 5376, 4096, True), (2, 22000, 4096, False), (1, 40000, 4096, False)])
+def test_two_streams_at_once(M, N, K, gated):
+    x, codes, grid, b, r = dev(*fused_inputs(M, N, K, gated, F16, F16, seed=3))
+
+    def call():
+        return dmm.decode_matmul_fused(x, codes, grid, 0.02, bias=b, activation="silu", gated=gated, residual=r)
+
+    want = call()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
