@@ -32,12 +32,37 @@ __device__ __forceinline__ float epi_sigmoid(float z)
 // 0.5 z (1 + tanh(u)) = z / (1 + exp(-2 u)), u = sqrt(2 / pi) (z + 0.044715 z^3): 2 u
 __device__ __forceinline__ float epi_tanh_arg(float z) { return 1.59576912160573071176f * __builtin_fmaf(0.044715f * z * z, z, z); }
 
+// z Phi(z) = max(z, 0) - a Phi(-a), a = |z|: nothing cancels for z < 0, where 0.5 z (1 + erf(z / sqrt 2)) loses all its digits
+// by -6.  Phi(-a) = exp(-a^2 / 2) Q(a); Q, the normal distribution's tail over its density (times 1 / sqrt(2 pi)), falls
+// slowly and is t P(t) with t = 1 / (1 + 0.35 a), P of degree 8 fitted for the least relative error over 0 <= a <= 14.5 (3.2e-8).  a^2 is
+// split into a rounded square and what that lost, and so is its product with -log2(e) / 2.  About ten half steps of the tail; 5 %
+// less time than erff for 2048 x 11008 outputs of K = 4096 (249 -> 236 us).
+__device__ __forceinline__ float epi_gelu(float z)
+{
+    const float a = __builtin_fminf(__builtin_fabsf(z), 40.f);   // far past the smallest float: no inf * 0
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.35f, a, 1.0f));
+    float q = -0.0291580297f;
+    q = __builtin_fmaf(q, t, 0.144031614f);
+    q = __builtin_fmaf(q, t, -0.255840391f);
+    q = __builtin_fmaf(q, t, 0.159321249f);
+    q = __builtin_fmaf(q, t, -0.023213394f);
+    q = __builtin_fmaf(q, t, 0.105552927f);
+    q = __builtin_fmaf(q, t, 0.119821183f);
+    q = __builtin_fmaf(q, t, 0.139863536f);
+    q = __builtin_fmaf(q, t, 0.139621302f) * t;
+    constexpr float kHalfLog2e = 0.721347510814666748047f, kHalfLog2eLo = 9.62981495563308734435e-9f, kLn2 = 0.693147182464599609375f;
+    const float s = a * a, t2 = s * -kHalfLog2e;
+    const float lost = __builtin_fmaf(s, -kHalfLog2e, -t2) - __builtin_fmaf(__builtin_fmaf(a, a, -s), kHalfLog2e, s * kHalfLog2eLo);
+    const float p = __builtin_amdgcn_exp2f(t2);
+    return (z > 0.f ? z : 0.f * z) - a * q * __builtin_fmaf(p, lost * kLn2, p);   // 0 * z: keeps NaN, and makes one of -inf
+}
+
 __device__ __forceinline__ float epi_act(float z, int act)
 {
     switch (act) {
         case DMM_ACT_RELU: return z < 0.f ? 0.f : z;   // keeps NaN
         case DMM_ACT_SILU: return z * epi_sigmoid(z);
-        case DMM_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752440f));
+        case DMM_ACT_GELU: return epi_gelu(z);
         case DMM_ACT_GELU_TANH: return z * epi_sigmoid(epi_tanh_arg(z));
         default: return z;
     }
@@ -122,7 +147,7 @@ __device__ __forceinline__ void epi_store1(const Epi &e, const EpiScale &sc, flo
     else reinterpret_cast<half_t *>(e.y)[i] = (half_t)z;
 }
 
-// The activation of four values side by side, which hides the latency of the exponentials.  kSmall: erf, by far the
+// The activation of four values side by side, which hides the latency of the exponentials.  kSmall: GELU, by far the
 // longest, one value after the other in a loop (the vector turned by one element each time), for kernels that
 // have no registers to spare.
 template <bool kSmall>

@@ -439,13 +439,14 @@ inline void host_store(void *p, int64_t i, int type, float v)
     else reinterpret_cast<half_t *>(p)[i] = (half_t)v;
 }
 
+// The two GELUs in 64 bits: in 32, their arguments' roundings would show in the tails.
 inline float host_act(float z, int act)
 {
     switch (act) {
         case DMM_ACT_RELU: return z < 0.f ? 0.f : z;
         case DMM_ACT_SILU: return z / (1.f + expf(-z));
-        case DMM_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752440f));
-        case DMM_ACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286535588f * (z + 0.044715f * z * z * z)));
+        case DMM_ACT_GELU: return (float)(0.5 * z * erfc(z * -0.70710678118654752440));
+        case DMM_ACT_GELU_TANH: return (float)(z / (1.0 + exp(-1.59576912160573071176 * (z + 0.044715 * z * z * z))));
         default: return z;
     }
 }
