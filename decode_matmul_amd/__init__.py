@@ -127,6 +127,17 @@ def decode(codes, grid):
     return _ext().decode(codes, grid)
 
 
+def _scale_pair(scale, gated, what):
+    """The scales of the two halves of a gated call; the same number twice unless they come as a pair."""
+    if not isinstance(scale, (tuple, list)):
+        return (float(scale),) * 2
+    if not gated:
+        raise RuntimeError("%s: a pair of scales is for a gated call" % what)
+    if len(scale) != 2:
+        raise RuntimeError("%s: a pair of scales is (gate, up), got %d values" % (what, len(scale)))
+    return float(scale[0]), float(scale[1])
+
+
 def decode_matmul_fused(x, codes, grid, scale, *, bias=None, activation="none", gated=False, residual=None, out_dtype=None):
     """`decode_matmul` with an epilogue, fp32 until one rounding at the store:
 
@@ -137,9 +148,7 @@ def decode_matmul_fused(x, codes, grid, scale, *, bias=None, activation="none", 
     x half [M, K]; bias (one value per row of codes) and residual [M, N] half or float32; activation "none",
     "relu", "silu", "gelu" (erf) or "gelu_tanh"; out_dtype float16 (default) or float32.  scale: a number, or for a gated
     call a pair (gate, up).  No gradient: an input that requires one is refused."""
-    scale, scale_up = (float(s) for s in scale) if isinstance(scale, (tuple, list)) else (float(scale),) * 2
-    if scale != scale_up and not gated:
-        raise RuntimeError("decode_matmul_fused: a pair of scales is for a gated call")
+    scale, scale_up = _scale_pair(scale, gated, "decode_matmul_fused")
     return _ext().decode_matmul_fused(x, codes, grid, scale, scale_up, bias, activation, bool(gated), residual,
                                       out_dtype or _torch.float16)
 

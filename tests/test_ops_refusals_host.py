@@ -44,3 +44,24 @@ def test_residual_that_overlaps_the_output_is_refused():
         assert call(host, y, 1, y, 1) == 0
         assert call(host, y + 2 * M * N, 0, y, 0) == 0          # side by side
         assert call(host, y - 2 * M * N, 0, y, 1) == 0
+
+
+# ----------------------------------------------------------------- scales
+def test_a_scale_that_is_nan_shows_in_the_result():
+    x, codes, grid, _, _ = fused_inputs(2, 8, 64, False, None, None, seed=1)
+    assert torch.isnan(dmm.decode_matmul_fused(x, codes, grid, math.nan)).all()
+    y = dmm.decode_matmul_fused(x, codes, grid, (math.nan, 1.0), gated=True)
+    assert torch.isnan(y).all() and y.shape == (2, 4)
+
+
+def test_a_pair_of_scales_is_for_a_gated_call_whatever_its_values():
+    x, codes, grid, _, _ = fused_inputs(2, 8, 64, False, None, None, seed=1)
+    for pair in ((0.5, 0.5), [0.5, 0.25], (math.nan, math.nan)):
+        with pytest.raises(RuntimeError, match="pair of scales is for a gated call"):
+            dmm.decode_matmul_fused(x, codes, grid, pair)
+    for bad in ((0.5,), (0.5, 0.5, 0.5), ()):
+        with pytest.raises(RuntimeError, match="pair of scales is"):
+            dmm.decode_matmul_fused(x, codes, grid, bad, gated=True)
+    for pair in ((0.5, 0.25), [0.5, 0.25]):
+        y = dmm.decode_matmul_fused(x, codes, grid, pair, gated=True, out_dtype=F32)
+        assert_within(y, *product64(x.double(), decode64(codes, grid), pair, None, True, "none", None, F32))
