@@ -147,7 +147,7 @@ def decode_matmul_fused(x, codes, grid, scale, *, bias=None, activation="none", 
 
     x half [M, K]; bias (one value per row of codes) and residual [M, N] half or float32; activation "none",
     "relu", "silu", "gelu" (erf) or "gelu_tanh"; out_dtype float16 (default) or float32.  scale: a number, or for a gated
-    call a pair (gate, up).  No gradient: an input that requires one is refused."""
+    call a pair (gate, up).  No gradient: an input that requires one, or carries a forward-mode tangent, is refused."""
     scale, scale_up = _scale_pair(scale, gated, "decode_matmul_fused")
     return _ext().decode_matmul_fused(x, codes, grid, scale, scale_up, bias, activation, bool(gated), residual,
                                       out_dtype or _torch.float16)

@@ -11,6 +11,7 @@
 // synchronisation and no exit() on error (a non-zero status becomes an exception); the
 // GIL is released around the launch.
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -245,10 +246,13 @@ typedef c10::optional<torch::Tensor> MaybeTensor;
 
 #define DMM_CHECK_SAME_DEVICE(t, dev) TORCH_CHECK((t).device() == (dev), #t " must be on ", (dev), " like x")
 
+// A gradient is asked for by requires_grad, or forward in a tangent beside the value (which lives under no_grad too).
 void check_no_grad(const torch::Tensor &t, const char *what, const char *name)
 {
     TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what, ": ", name,
                 " requires a gradient, which this operator does not compute; call it under torch.no_grad() or detach the input");
+    TORCH_CHECK(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(/*level=*/0).defined()), what, ": ", name,
+                " carries a tangent of forward-mode differentiation, a gradient which this operator does not compute; unpack or detach the input");
 }
 
 void check_device(const torch::Device &d, const char *what)

@@ -65,3 +65,55 @@ def test_a_pair_of_scales_is_for_a_gated_call_whatever_its_values():
     for pair in ((0.5, 0.25), [0.5, 0.25]):
         y = dmm.decode_matmul_fused(x, codes, grid, pair, gated=True, out_dtype=F32)
         assert_within(y, *product64(x.double(), decode64(codes, grid), pair, None, True, "none", None, F32))
+
+
+# ----------------------------------------------------------------- gradients
+def calls():
+    """(name of the input, call with it replaced): every input that could carry a gradient."""
+    x, codes, grid, b, r = fused_inputs(2, 8, 64, False, F16, F16, seed=1)
+    gx, gcodes, ggrid, offsets, rows, gb = grouped_inputs((2, 3), 4, 8, 64, False, F16, True, seed=3)
+    y, slots, w, res = torch.ones(4, 8, dtype=F16), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, 2), torch.ones(3, 8)
+    fused = {"x": x, "grid": grid, "bias": b, "residual": r}
+    for name, t in fused.items():
+        def call(v, n=name):
+            a = dict(fused, **{n: v})
+            return dmm.decode_matmul_fused(a["x"], codes, a["grid"], 0.1, bias=a["bias"], residual=a["residual"])
+        yield "fused", name, t, call
+    grouped = {"x": gx, "grid": ggrid, "bias": gb, "scale": torch.ones(2), "out": torch.zeros(5, 8, dtype=F16)}
+    for name, t in grouped.items():
+        def call(v, n=name):
+            a = dict(grouped, **{n: v})
+            return dmm.decode_matmul_grouped(a["x"], gcodes, a["grid"], a["scale"], offsets, rows=rows, bias=a["bias"], out=a["out"])
+        yield "grouped", name, t, call
+    yield "route", "logits", torch.ones(3, 8), lambda v: dmm.route_experts(v, 2)
+    combine = {"y": y, "weights": w, "residual": res}
+    for name, t in combine.items():
+        def call(v, n=name):
+            a = dict(combine, **{n: v})
+            return dmm.combine_experts(a["y"], slots, a["weights"], residual=a["residual"])
+        yield "combine", name, t, call
+
+
+CALLS = list(calls())
+
+
+@pytest.mark.parametrize("op,name,t,call", CALLS, ids=["%s-%s" % c[:2] for c in CALLS])
+def test_an_input_that_asks_for_a_gradient_is_refused(op, name, t, call):
+    import torch.autograd.forward_ad as fwd
+    call(t)
+    with pytest.raises(RuntimeError, match="%s requires a gradient" % name):
+        call(t.clone().requires_grad_())
+    with torch.no_grad():
+        call(t.clone().requires_grad_())
+    with fwd.dual_level():
+        dual = fwd.make_dual(t.clone(), torch.ones_like(t))
+        with pytest.raises(RuntimeError, match="%s carries a tangent" % name):
+            call(dual)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="%s carries a tangent" % name):      # tangents live on under it
+            call(dual)
+        call(fwd.unpack_dual(dual).primal)
+        with torch.inference_mode():                                                                  # where they do not
+            call(dual)
+    if name != "out":                                          # torch.func's transforms: an error, never a wrong gradient
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda v: call(v), (t,), (torch.ones_like(t),))
