@@ -127,15 +127,22 @@ def decode(codes, grid):
     return _ext().decode(codes, grid)
 
 
+def _number(scale, what):
+    """A scale as a number; a tensor of one value is read (which waits for its device)."""
+    if isinstance(scale, _torch.Tensor):
+        _ext().check_no_grad(scale, what, "scale")
+    return float(scale)
+
+
 def _scale_pair(scale, gated, what):
     """The scales of the two halves of a gated call; the same number twice unless they come as a pair."""
     if not isinstance(scale, (tuple, list)):
-        return (float(scale),) * 2
+        return (_number(scale, what),) * 2
     if not gated:
         raise RuntimeError("%s: a pair of scales is for a gated call" % what)
     if len(scale) != 2:
         raise RuntimeError("%s: a pair of scales is (gate, up), got %d values" % (what, len(scale)))
-    return float(scale[0]), float(scale[1])
+    return _number(scale[0], what), _number(scale[1], what)
 
 
 def decode_matmul_fused(x, codes, grid, scale, *, bias=None, activation="none", gated=False, residual=None, out_dtype=None):

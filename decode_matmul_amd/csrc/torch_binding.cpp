@@ -539,6 +539,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("x"), pybind11::arg("packed"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("N"));
     m.def("decode", &decode, "Decode codes [N, K/8] to the dense half matrix [N, K]",
           pybind11::arg("codes"), pybind11::arg("grid"));
+    m.def("check_no_grad", [](const torch::Tensor &t, const std::string &what, const std::string &name) { check_no_grad(t, what.c_str(), name.c_str()); },
+          "RuntimeError if t asks for a gradient", pybind11::arg("t"), pybind11::arg("what"), pybind11::arg("name"));
     m.def("decode_matmul_fused", &decode_matmul_fused, "decode_matmul with bias, activation, gate and residual in its epilogue",
           pybind11::arg("x"), pybind11::arg("codes"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("scale_up"),
           pybind11::arg("bias"), pybind11::arg("activation"), pybind11::arg("gated"), pybind11::arg("residual"),

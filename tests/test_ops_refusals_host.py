@@ -117,3 +117,18 @@ def test_an_input_that_asks_for_a_gradient_is_refused(op, name, t, call):
     if name != "out":                                          # torch.func's transforms: an error, never a wrong gradient
         with pytest.raises(RuntimeError):
             torch.func.jvp(lambda v: call(v), (t,), (torch.ones_like(t),))
+
+
+def test_a_scale_tensor_that_asks_for_a_gradient_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x, codes, grid, _, _ = fused_inputs(2, 8, 64, False, None, None, seed=1)
+    s = torch.tensor(0.5, requires_grad=True)
+    want = dmm.decode_matmul_fused(x, codes, grid, 0.5)
+    for scale, gated in ((s, False), ((s, 0.5), True), ((0.5, s), True)):
+        with pytest.raises(RuntimeError, match="scale requires a gradient"):
+            dmm.decode_matmul_fused(x, codes, grid, scale, gated=gated)
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="scale carries a tangent"):
+        dmm.decode_matmul_fused(x, codes, grid, fwd.make_dual(s.detach(), torch.tensor(1.0)))
+    with torch.no_grad():
+        assert torch.equal(dmm.decode_matmul_fused(x, codes, grid, s), want)
+    assert torch.equal(dmm.decode_matmul_fused(x, codes, grid, s.detach()), want)
