@@ -166,13 +166,13 @@ def decode_matmul_grouped(x, codes, grid, scale, offsets, *, rows=None, bias=Non
     is made with codes[e] from x[rows[p]] (rows=None: x[p]).
 
     codes [E, N, K/8] (gated: [E, 2 N, K/8]), bias [E, ...] one value per row of codes, scale a number, float32 [E], or
-    for a gated call float32 [E, 2]; offsets int32 [E + 1] and rows int32 [R] live on x's device and are not read by the
+    for a gated call a pair (gate, up) or float32 [E, 2]; offsets int32 [E + 1] and rows int32 [R] live on x's device and are not read by the
     host (`route_experts` makes both).  An entry of rows outside x stands for a row of zeros.  Rows from
     offsets[E] on are not written: in `out` (optional, [R, N], no memory shared with an input) they stay as they were, in a
     result allocated here their content is undefined."""
-    scales = scale if isinstance(scale, _torch.Tensor) else None
-    return _ext().decode_matmul_grouped(x, codes, grid, 1.0 if scales is not None else float(scale), scales, offsets, rows, bias,
-                                        activation, bool(gated), out_dtype or (out.dtype if out is not None else _torch.float16), out)
+    scales, number = (scale, (1.0, 1.0)) if isinstance(scale, _torch.Tensor) else (None, _scale_pair(scale, gated, "decode_matmul_grouped"))
+    return _ext().decode_matmul_grouped(x, codes, grid, *number, scales, offsets, rows, bias, activation, bool(gated),
+                                        out_dtype or (out.dtype if out is not None else _torch.float16), out)
 
 
 Routing = _collections.namedtuple("Routing", "weights experts offsets rows slots")

@@ -362,8 +362,8 @@ bool share_memory(const torch::Tensor &a, const torch::Tensor &b)   // both cont
     return a.nbytes() > 0 && b.nbytes() > 0 && pa < pb + b.nbytes() && pb < pa + a.nbytes();
 }
 
-torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch::Tensor grid, double scale, MaybeTensor scales,
-                                    torch::Tensor offsets, MaybeTensor rows, MaybeTensor bias, const std::string &activation,
+torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch::Tensor grid, double scale, double scale_up,
+                                    MaybeTensor scales, torch::Tensor offsets, MaybeTensor rows, MaybeTensor bias, const std::string &activation,
                                     bool gated, torch::ScalarType out_dtype, MaybeTensor out)
 {
     check_weights(x, codes, grid, 3, "decode_matmul_grouped");
@@ -384,7 +384,8 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
     dmm_epilogue ep{};
     ep.activation = activation_of(activation);
     ep.gated = gated;
-    ep.scale = ep.scale_up = static_cast<float>(scale);
+    ep.scale = static_cast<float>(scale);
+    ep.scale_up = static_cast<float>(scale_up);
     ep.out_type = out_type_of(out_dtype);
     int scale_cols = 1;
     if (scales) {
@@ -392,7 +393,7 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
         DMM_CHECK_CONTIGUOUS(*scales);
         TORCH_CHECK(scales->scalar_type() == torch::kFloat &&
                         (scales->dim() == 1 || (gated && scales->dim() == 2 && scales->size(1) == 2)) && scales->size(0) == E,
-                    "scale must be a number, float32 [E], or float32 [E, 2] for a gated call");
+                    "scale must be a number, float32 [E], or for a gated call a pair of numbers or float32 [E, 2]");
         check_no_grad(*scales, "decode_matmul_grouped", "scale");
         scale_cols = static_cast<int>(scales->dim());
     }
@@ -546,7 +547,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
           pybind11::arg("bias"), pybind11::arg("activation"), pybind11::arg("gated"), pybind11::arg("residual"),
           pybind11::arg("out_dtype"));
     m.def("decode_matmul_grouped", &decode_matmul_grouped, "decode_matmul_fused per expert, rows grouped by expert",
-          pybind11::arg("x"), pybind11::arg("codes"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("scales"),
+          pybind11::arg("x"), pybind11::arg("codes"), pybind11::arg("grid"), pybind11::arg("scale"), pybind11::arg("scale_up"), pybind11::arg("scales"),
           pybind11::arg("offsets"), pybind11::arg("rows"), pybind11::arg("bias"), pybind11::arg("activation"), pybind11::arg("gated"),
           pybind11::arg("out_dtype"), pybind11::arg("out"));
     m.def("route_experts", &route_experts, "The k largest logits per row, their weights, and the rows sorted by expert",

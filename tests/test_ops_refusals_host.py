@@ -132,3 +132,18 @@ def test_a_scale_tensor_that_asks_for_a_gradient_is_refused():
     with torch.no_grad():
         assert torch.equal(dmm.decode_matmul_fused(x, codes, grid, s), want)
     assert torch.equal(dmm.decode_matmul_fused(x, codes, grid, s.detach()), want)
+
+
+def test_grouped_takes_a_pair_of_scales_as_fused_does():
+    x, codes, grid, offsets, rows, b = grouped_inputs((2, 0, 3), 4, 8, 64, True, F16, True, seed=3)
+    pair = (0.25, 0.125)
+    y = dmm.decode_matmul_grouped(x, codes, grid, pair, offsets, rows=rows, bias=b, activation="silu", gated=True, out_dtype=F32)
+    assert_within(y, *grouped64(x, codes, grid, torch.tensor([pair] * 3), offsets, rows, b, True, "silu", F32, 8))
+    assert torch.equal(y, dmm.decode_matmul_grouped(x, codes, grid, torch.tensor([pair] * 3), offsets, rows=rows, bias=b, activation="silu", gated=True,
+                                                    out_dtype=F32))
+    with pytest.raises(RuntimeError, match="decode_matmul_grouped: a pair of scales is for a gated call"):
+        dmm.decode_matmul_grouped(x, codes, grid, pair, offsets, rows=rows)
+    with pytest.raises(RuntimeError, match="pair of scales is"):
+        dmm.decode_matmul_grouped(x, codes, grid, (0.5,) * 3, offsets, rows=rows, gated=True)
+    with pytest.raises(RuntimeError, match="scale must be"):
+        dmm.decode_matmul_grouped(x, codes, grid, torch.ones(2), offsets, rows=rows, gated=True)
