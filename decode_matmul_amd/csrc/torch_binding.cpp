@@ -431,6 +431,8 @@ torch::Tensor decode_matmul_grouped(torch::Tensor x, torch::Tensor codes, torch:
                                                     offsets.data_ptr(), &ep, y.data_ptr(), R, E, N, K, stream);
     }
     check_status(st, "decode_matmul_grouped");
+    // what autograd may have saved of `out` has changed
+    if (out && !y.is_inference()) y.unsafeGetTensorImpl()->bump_version();
     return y;
 }
 

@@ -147,3 +147,16 @@ def test_grouped_takes_a_pair_of_scales_as_fused_does():
         dmm.decode_matmul_grouped(x, codes, grid, (0.5,) * 3, offsets, rows=rows, gated=True)
     with pytest.raises(RuntimeError, match="scale must be"):
         dmm.decode_matmul_grouped(x, codes, grid, torch.ones(2), offsets, rows=rows, gated=True)
+
+
+def test_grouped_out_counts_as_written():
+    """A product that saved `out` for its gradient: an error afterwards, not a gradient of other values."""
+    x, codes, grid, offsets, rows, _ = grouped_inputs((2, 3), 4, 8, 64, False, None, True, seed=3)
+    out, w = torch.ones(5, 8, dtype=F16), torch.ones(5, 8, dtype=F16, requires_grad=True)
+    product = (w * out).sum()
+    dmm.decode_matmul_grouped(x, codes, grid, 0.1, offsets, rows=rows, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
+    with torch.inference_mode():
+        out = torch.ones(5, 8, dtype=F16)
+    dmm.decode_matmul_grouped(x, codes, grid, 0.1, offsets, rows=rows, out=out)          # has no version
