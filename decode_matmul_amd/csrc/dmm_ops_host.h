@@ -283,10 +283,12 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
     if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
-    const bool rows_ok = ops_jobs_fit(g, 4, e.N), mid_ok = ops_jobs_fit(g, kMidRows, e.N);
+    // The kernels whose loads add the offset of a row inside a tile (of 16 rows of W, of 32 of x) to the tile's take K up to 2^23, as
+    // the plain product's do: the sums stay below 2^32.  Longer ones go to the matrix-matrix kernel, whose lanes have one offset.
+    const bool k_ok = K <= (1 << 23), rows_ok = k_ok && ops_jobs_fit(g, 4, e.N), mid_ok = k_ok && ops_jobs_fit(g, kMidRows, e.N);
     const int cus = cu_count();
     // One row of a matrix: the batch-1 kernels' bodies
-    const bool one_row = force < 0 && !g.offsets && g.R == 1 && (K & 255) == 0;
+    const bool one_row = force < 0 && k_ok && !g.offsets && g.R == 1 && (K & 255) == 0;
     if (!kGated && one_row && (e.N & 3) == 0 && ((int64_t)e.N + 15) / 16 <= cus && ops_stream_lds(K) <= kLdsMax)
         return launch_ops_stream(x, codes, grid, g, e, K, s);
     if (one_row && !e.out_f32 && ops_share(e.N, kGated) <= 8 && gemv_q8_enabled()) return launch_ops_q8d<kGated>(x, codes, grid, g, e, K, s);
@@ -298,7 +300,7 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
     // 16.8, 12288 -> 8192 9.4 / 9.9, 28672 -> 8192 16.4 / 17.2, 4096 -> 2 x 11008 8.72 / 9.35, 8192 -> 2 x 28672 30.5 / 35.5).  By
     // expert where few experts have a row and the codes are many (2 x 11008 x 4096, 8 experts, 1 row 12.7, 16-bit 14.4; 2 rows
     // 18.9 / 21.1; but 4 rows 24.7 / 20.6).
-    const bool rows8_ok = ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (e.residual != e.y || ops_redo_by_number(g, e.N, cus));
+    const bool rows8_ok = k_ok && ops_jobs_fit(g, 2, e.N) && !e.out_f32 && (e.residual != e.y || ops_redo_by_number(g, e.N, cus));
     const int64_t share = ops_share(e.N, kGated);
     const bool rows8_pays = g.offsets ? (g.R <= 2 || 4 * (int64_t)g.R <= g.E) && K >= 4096 &&
                                             std::min<int64_t>(g.R, g.E) * rows * (K >> 2) >= (20LL << 20)

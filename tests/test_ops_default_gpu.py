@@ -235,3 +235,24 @@ def test_two_streams_at_once(M, N, K, gated):
             outs.append(call())
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+# ----------------------------------------------------------------- long K
+# the batch-1 body past the longest x of the plain product's batch-1 kernels, the jobs' kernel, and the last K of both
+@pytest.mark.parametrize("M,N,gated", [(1, 8190, False), (1, 4100, True), (2, 12300, False)])
+@pytest.mark.parametrize("K,first", [(40960, 5088), (65536, 0), (65536, 4000), (65536, 8160)])
+def test_long_k_sees_every_term(M, N, gated, K, first):
+    check_terms(M, N, K, gated, first, 32)
+
+
+@pytest.mark.parametrize("kernel", [-1, 1, 2, 3, 4, 5], ids=["auto", "rows", "gemm", "split", "rows8", "mid"])
+@pytest.mark.parametrize("K", [1 << 23, (1 << 23) + 64, (1 << 23) + 16])
+@pytest.mark.parametrize("M", [1, 2, 3, 17])
+def test_k_at_and_past_the_longest_of_the_row_kernels(M, K, kernel):
+    """x is zero but for 256 k near the end of K; both sides of the limit."""
+    capi.lib().dmm_set_ops_kernel(kernel)
+    first = K // 8 - 40
+    c = Case(M, 20, K, 5, first, 32)
+    b, left = cancelling(c)
+    y = dmm.decode_matmul_fused(*dev(c.x, c.codes, c.grid), 1.0, bias=b.to(DEV))
+    check_cancelled(y, left.expand(M, 20), c.tol())
