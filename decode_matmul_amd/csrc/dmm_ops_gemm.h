@@ -24,9 +24,9 @@ struct GemmOpsPlace {
     int m0, m_end, n0, expert;
     const Groups &g;
     const Epi &epi;
-    __device__ __forceinline__ int x_base(int m, int K) const
+    __device__ __forceinline__ int x_base(int m, int K) const   // no list: from the block's first row on
     {
-        const int t = group_row(g, m);
+        const int t = g.rows ? group_row(g, m) : m - m0;
         return t < 0 ? kGrOut : t * K * 2;
     }
     __device__ __forceinline__ int w_row(int i, int wave, int l32) const
@@ -120,7 +120,10 @@ __global__ __launch_bounds__(256) void ops_gemm_kernel(const uint16_t *__restric
     typedef GemmOpsPlace<kGated> Place;
     const Place p{first, end, (int)blockIdx.y * Place::kOutN, expert, g, epi};
     const int rows = kGated ? 2 * epi.N : epi.N;
-    gemm_reg_body<TM, false, false>(p, x, (int64_t)g.T * K * 2, codes + (int64_t)expert * rows * (K >> 3), rows, grid, K, 1);
+    // Without a list the block's rows of x follow each other: 31-bit offsets from its first one, wherever that lies.
+    const int64_t x_first = g.rows ? 0 : first, x_bytes = (g.T - x_first) * K * 2;
+    gemm_reg_body<TM, false, false>(p, x + x_first * K, x_bytes < INT32_MAX ? x_bytes : INT32_MAX,
+                                    codes + (int64_t)expert * rows * (K >> 3), rows, grid, K, 1);
 }
 
 // y = epilogue(sum over z of part[z]): part [splits][M][N or 2 N] fp32, added in a fixed order.  One thread per four outputs.

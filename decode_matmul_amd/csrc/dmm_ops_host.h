@@ -64,12 +64,17 @@ int run_ops_generic(const void *x, const void *codes, const void *grid, const Gr
                   (const uint16_t *)codes, grid, g, e, K);
 }
 
-// the matrix unit's kernels: 16-byte loads at 4-byte aligned places, 31-bit offsets into x and one expert's codes
+// the matrix unit's kernels: 16-byte loads at 4-byte aligned places, 31-bit offsets into one expert's codes
 bool ops_mfma_ok(const void *x, const void *codes, const void *grid, const Groups &g, int64_t rows, int64_t K)
 {
     return K >= 16 && (K & 15) == 0 && aligned(x, 16) && aligned(codes, 16) && aligned(grid, 16) && g.T > 0 &&
-           (int64_t)g.T * K * 2 < (1LL << 31) && rows * (K >> 2) < (1LL << 31) && rows <= 65535LL * 128;
+           rows * (K >> 2) < (1LL << 31) && rows <= 65535LL * 128;
 }
+
+// and into x: all of them where x is below 2 GiB; the matrix-matrix kernel has its offsets from the first of up to 128 rows
+// of a block if these follow each other (139266 rows of 8192, past 2 GiB, to 2048: 5.4 ms, the catch-all 760)
+inline bool ops_x_near(const Groups &g, int64_t K) { return (int64_t)g.T * K * 2 < (1LL << 31); }
+inline bool ops_x_by_block(const Groups &g, int64_t K) { return !g.rows && 128 * K * 2 < (1LL << 31); }
 
 template <int TM, bool kGated>
 int launch_ops_gemm(const void *x, const void *codes, const void *grid, const Groups &g, const Epi &e, int64_t K, hipStream_t s)
@@ -282,7 +287,9 @@ int run_ops(const void *x, const void *codes, const void *grid, const Groups &g,
 {
     const int64_t rows = kGated ? 2 * (int64_t)e.N : e.N;
     const int force = g_ops_kernel.load(std::memory_order_relaxed);
-    if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K)) return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
+    if (force == kOpsGeneric || !ops_mfma_ok(x, codes, grid, g, rows, K) || !(ops_x_near(g, K) || ops_x_by_block(g, K)))
+        return run_ops_generic<kGated>(x, codes, grid, g, e, K, s);
+    if (!ops_x_near(g, K)) return run_ops_gemm<kGated>(x, codes, grid, g, e, K, s);
     // The kernels whose loads add the offset of a row inside a tile (of 16 rows of W, of 32 of x) to the tile's take K up to 2^23, as
     // the plain product's do: the sums stay below 2^32.  Longer ones go to the matrix-matrix kernel, whose lanes have one offset.
     const bool k_ok = K <= (1 << 23), rows_ok = k_ok && ops_jobs_fit(g, 4, e.N), mid_ok = k_ok && ops_jobs_fit(g, kMidRows, e.N);

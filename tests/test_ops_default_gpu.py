@@ -8,7 +8,7 @@ import decode_matmul_amd as dmm
 from decode_matmul_amd import capi
 from gpu_util import DEV
 from ops_terms import Case, cancelling, grouped8
-from ops_util import assert_within, check_routing, combine64, decode64, fused_inputs, product64, weights
+from ops_util import assert_within, check_routing, combine64, decode64, fused_inputs, grouped_inputs, product64, weights
 
 pytestmark = pytest.mark.gpu
 F16, F32 = torch.float16, torch.float32
@@ -256,3 +256,37 @@ def test_k_at_and_past_the_longest_of_the_row_kernels(M, K, kernel):
     b, left = cancelling(c)
     y = dmm.decode_matmul_fused(*dev(c.x, c.codes, c.grid), 1.0, bias=b.to(DEV))
     check_cancelled(y, left.expand(M, 20), c.tol())
+
+
+# ----------------------------------------------------------------- x of 2 GiB and more
+def test_x_past_2_gib():
+    """Rows on both sides of 2^31 bytes, dense and by expert, in their order and (the catch-all) through a list; blocks that begin
+    anywhere, a last one that is cut."""
+    T, N, K = 139269, 80, 8192                     # row 131072 begins at 2^31
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.empty(T, K, dtype=F16, device=DEV)
+    for i in range(0, T, 8192):
+        x[i:i + 8192] = torch.randn(min(8192, T - i), K, generator=gen, device=DEV)
+    pick = torch.tensor([0, 1, 127, 128, 65535, 65536, 131071, 131072, 131073, 131200, 139264, T - 1])
+    xs = x[pick.to(DEV)].cpu().double()
+    s = 1 / math.sqrt(K)
+    for gated in (False, True):
+        _, codes, grid, b, _ = fused_inputs(1, N, K, gated, F32, None, 4)
+        r = torch.randn(T, N, generator=gen, device=DEV).half()
+        y = dmm.decode_matmul_fused(x, *dev(codes, grid), s, bias=b.to(DEV), activation="silu", gated=gated, residual=r)
+        assert_within(y[pick.to(DEV)], *product64(xs, decode64(codes, grid), (s, s), b, gated, "silu", r[pick.to(DEV)].cpu(), F16))
+    ends = (0, 100, 131071, 131071, T - 3)         # the last three rows belong to no expert
+    _, codes, grid, _, _, b = grouped_inputs((1, 1, 1, 1), 1, N, K, True, F16, False, 5)
+    out = torch.full((T, N), 7.0, dtype=F16, device=DEV)
+    dmm.decode_matmul_grouped(x, *dev(codes, grid), s, torch.tensor(ends, dtype=torch.int32, device=DEV), bias=b.to(DEV), activation="gelu", gated=True, out=out)
+    for p, xp in zip(pick.tolist(), xs):
+        if p >= ends[-1]:
+            assert torch.all(out[p] == 7.0)
+            continue
+        e = max(i for i in range(4) if ends[i] <= p < ends[i + 1])
+        assert_within(out[p:p + 1], *product64(xp[None], decode64(codes[e], grid), (s, s), b[e], True, "gelu", None, F16), "row %d" % p)
+    rows = pick.int().flip(0).contiguous()
+    y = dmm.decode_matmul_grouped(x, *dev(codes, grid), s, torch.tensor([0, 5, 5, 12, 12], dtype=torch.int32, device=DEV), rows=rows.to(DEV),
+                                  bias=b.to(DEV), gated=True)
+    for lo, hi, e in ((0, 5, 0), (5, 12, 2)):
+        assert_within(y[lo:hi], *product64(xs.flip(0)[lo:hi], decode64(codes[e], grid), (s, s), b[e], True, "none", None, F16))
