@@ -8,7 +8,7 @@ import decode_matmul_amd as dmm
 from decode_matmul_amd import capi
 from gpu_util import DEV
 from ops_terms import Case, cancelling, grouped8
-from ops_util import assert_within, check_routing, combine64, decode64, fused_inputs, grouped_inputs, product64, weights
+from ops_util import assert_within, check_routing, combine64, decode64, fused_inputs, grouped64, grouped_inputs, product64, weights
 
 pytestmark = pytest.mark.gpu
 F16, F32 = torch.float16, torch.float32
@@ -290,3 +290,85 @@ def test_x_past_2_gib():
                                   bias=b.to(DEV), gated=True)
     for lo, hi, e in ((0, 5, 0), (5, 12, 2)):
         assert_within(y[lo:hi], *product64(xs.flip(0)[lo:hi], decode64(codes[e], grid), (s, s), b[e], True, "none", None, F16))
+
+
+# ----------------------------------------------------------------- corners of the ranges
+@pytest.fixture(params=[-1, 0, 1, 2, 3, 4, 5], ids=["auto", "generic", "rows", "gemm", "split", "rows8", "mid"])
+def kernel(request):
+    capi.lib().dmm_set_ops_kernel(request.param)
+    return request.param
+
+
+@pytest.mark.parametrize("K", [16, 32, 48, 80, 112, 144])
+@pytest.mark.parametrize("N,gated", [(1, False), (2, True), (3, False), (15, True), (18, False)])
+def test_short_k_and_few_columns(N, K, gated, kernel):
+    for M in (1, 2, 3, 9, 33, 70, 140):
+        x, codes, grid, b, r = fused_inputs(M, N, K, gated, F32, F16, M + N + K, coarse=True)
+        y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.1, bias=b.to(DEV), activation="gelu", gated=gated, residual=r.to(DEV))
+        assert_within(y, *product64(x.double(), decode64(codes, grid), (0.1, 0.1), b, gated, "gelu", r, F16), "M=%d" % M)
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_thousands_of_experts(gated, kernel):
+    """5000 experts, most without a row, of 16 columns and K = 48."""
+    E, N, K = 5000, 16, 48
+    counts = [0] * E
+    for e, n in ((0, 3), (63, 1), (64, 2), (1999, 40), (2047, 1), (3333, 130), (E - 1, 2)):
+        counts[e] = n
+    x, codes, grid, offsets, rows, b = grouped_inputs(tuple(counts), 9, N, K, gated, F16, True, 3, behind=4, coarse=True)
+    out = torch.full((rows.shape[0], N), 5.0, dtype=F16, device=DEV)
+    dmm.decode_matmul_grouped(*dev(x, codes, grid), 0.1, offsets.to(DEV), rows=rows.to(DEV), bias=b.to(DEV), gated=gated, out=out)
+    want, tol = grouped64(x, codes, grid, 0.1, offsets, rows, b, gated, "none", F16, N)
+    assert torch.all(out[-4:] == 5.0)
+    assert_within(out[:-4], want[:-4], tol[:-4])
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_jobs_behind_the_numbered_ones_are_done_again(gated):
+    """Forced onto 8-bit operands, 78 jobs per workgroup: infinities early and late, the rows beside them unharmed."""
+    M, N, K = 40000, 16, 256
+    x, codes, grid, b, r = fused_inputs(M, N, K, gated, F16, F16, 3, coarse=True)
+    bad = [M - 1, M // 2, 140, 3]
+    x[bad, 100] = math.inf
+    capi.lib().dmm_set_ops_kernel(4)
+    y = dmm.decode_matmul_fused(*dev(x, codes, grid), 0.05, bias=b.to(DEV), gated=gated, residual=r.to(DEV)).cpu()
+    want, tol = product64(x.double(), decode64(codes, grid), (0.05, 0.05), b, gated, "none", r, F16)
+    keep = torch.ones(M, dtype=torch.bool)
+    keep[bad] = False
+    assert_within(y[keep], want[keep], tol[keep])
+    assert torch.equal(torch.isnan(y[bad]), torch.isnan(want[bad])) and not torch.isfinite(y[bad]).any()
+
+
+@pytest.mark.parametrize("M,N,gated", [(1, 200003, False), (2, 131075, False), (2, 70001, True)])
+def test_very_many_columns_see_every_term(M, N, gated):
+    check_terms(M, N, 2304, gated, 200, 32)
+
+
+@pytest.mark.parametrize("where", ["host", "gpu"])
+def test_nothing_to_do(where):
+    d = "cpu" if where == "host" else DEV
+    x, codes, grid, _, _ = (t.to(d) if t is not None else None for t in fused_inputs(2, 8, 64, False, None, None, 1))
+    assert dmm.decode_matmul_fused(x[:0], codes, grid, 1.0, residual=torch.empty(0, 8, device=d)).shape == (0, 8)
+    assert dmm.decode_matmul_fused(x, codes[:0], grid, 1.0, gated=True, bias=torch.empty(0, device=d)).shape == (2, 0)
+    offsets = torch.zeros(1, dtype=torch.int32, device=d)
+    assert dmm.decode_matmul_grouped(x, codes[None][:0], grid, 1.0, offsets).shape == (2, 8)
+    assert dmm.combine_experts(x[:, :0].contiguous(), torch.zeros(3, 2, dtype=torch.int32, device=d), torch.ones(3, 2, device=d)).shape == (3, 0)
+    r = dmm.route_experts(torch.zeros(0, 3, device=d), 3)
+    assert r.offsets.tolist() == [0] * 4 and r.rows.shape == (0,)
+
+
+@pytest.mark.parametrize("where", ["host", "gpu"])
+@pytest.mark.parametrize("E,k", [(5, 3), (300, 20)])
+def test_route_logit_of_plus_infinity(E, k, where):
+    """sigmoid: a weight like any other; softmax: inf - inf, NaN, as torch.softmax has it; chosen first either way."""
+    z = torch.randn(3, E, generator=torch.Generator().manual_seed(1))
+    z[1, 4] = math.inf
+    zd = z if where == "host" else z.to(DEV)
+    for normalize in (False, True):
+        r = dmm.route_experts(zd, k, scoring="sigmoid", normalize=normalize)
+        assert r.experts[1, 0] == 4 and torch.isfinite(r.weights).all()
+        top = torch.sigmoid(torch.sort(z.double(), dim=1, descending=True).values[:, :k])
+        want = top / top.sum(1, keepdim=True) if normalize else top
+        assert_within(r.weights, want, (E + 40) * 2.0 ** -24 * want)
+        r = dmm.route_experts(zd, k, normalize=normalize)
+        assert r.experts[1, 0] == 4 and torch.isnan(r.weights[1]).all() and torch.isfinite(r.weights[[0, 2]]).all()
