@@ -356,8 +356,9 @@ int dispatch_ops(const void *x, const void *codes, const void *grid, const Group
 // 0: no split
 int64_t ops_workspace_bytes(int64_t M, int64_t N, int64_t K, bool gated)
 {
+    if (M < kSplitKMinM || N < 1 || K < 64 || (K & 63) || M > 65535LL * 128 || N > INT32_MAX / 2 || K > INT32_MAX) return 0;   // first: no overflow below
     const int64_t rows = gated ? 2 * N : N;
-    if (M < kSplitKMinM || N < 1 || K < 64 || (K & 63) || M > 65535LL * 128 || !gemm_reg_ok(M, rows, K)) return 0;
+    if (!gemm_reg_ok(M, rows, K)) return 0;
     if (ops_dense_choice(M, N, K, gated, cu_count_or_default()) != kOpsGemm && g_ops_kernel.load(std::memory_order_relaxed) != kOpsSplit) return 0;
     const int splits = splitk_plan(M, rows, K, INT64_MAX, cu_count_or_default());
     return splits >= 2 ? (int64_t)splits * M * rows * 4 : 0;

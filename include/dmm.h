@@ -309,7 +309,9 @@ typedef struct dmm_epilogue {
 
 /* The product with an epilogue: y[M,N] from x half [M,K], codes [N,K/8] (gated: [2 N,K/8]), grid half [256,8], as
  * dmm_decode_matmul_f16 takes them; K % 8 == 0 is the only shape demand, K == 0 is an empty sum.  K % 16 == 0
- * with 16-byte aligned x, codes and grid runs on the matrix unit, everything else on the catch-all.
+ * with 16-byte aligned x, codes and grid runs on the matrix unit, everything else on the catch-all.  Where K is no multiple
+ * of 256 the matrix unit meets codes past a row's end with zeros for x: the grid has to be finite there (a value that is
+ * not may show in the results of a row of W that does not hold it).
  * The workspace is that of dmm_decode_matmul_ws_f16: dmm_fused_workspace_bytes bytes let a short x split K as far
  * as it would like, fewer (or NULL, 0) only limit the split. */
 int64_t dmm_fused_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated);
