@@ -166,5 +166,5 @@ def test_workspace_of_sizes_that_are_refused():
     """No split, so no workspace, for sizes the call itself refuses; their products do not fit 64 bits."""
     need = capi.lib().dmm_fused_workspace_bytes
     assert need(300, 4096, 11008, 0) > 0
-    for M, N, K, gated in ((32, 64, 1 << 60, 0), (32, 1 << 62, 64, 1), (64, 1 << 31, 1 << 40, 0), (1 << 40, 64, 64, 0), (17, 16, 1 << 62, 1)):
+    for M, N, K, gated in ((40, 16, 1 << 60, 1), (40, 16, (1 << 62) + 64, 0), (32, 1 << 62, 64, 1), (64, 1 << 31, 1 << 40, 0), (1 << 40, 64, 64, 0), (17, 16, 1 << 62, 1)):
         assert need(M, N, K, gated) == 0
