@@ -186,7 +186,9 @@ def route_experts(logits, k, *, scoring="softmax", normalize=True):
         experts  int32 [T, k]     -1: no choice (a logit of -inf or NaN is never chosen; such a weight is 0)
         offsets  int32 [E + 1]    first row of every expert, rows sorted by expert, then by token
         rows     int32 [T * k]    the token of every sorted row; -1 from offsets[E] on
-        slots    int32 [T, k]     the sorted row of every choice; -1: no choice"""
+        slots    int32 [T, k]     the sorted row of every choice; -1: no choice
+
+    The five share one allocation, which any of them keeps alive (clone one that is kept or saved by itself)."""
     return Routing(*_ext().route_experts(logits, int(k), scoring, bool(normalize)))
 
 

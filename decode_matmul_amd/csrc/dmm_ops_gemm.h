@@ -14,7 +14,7 @@
 //     back row by row: stores and the reads of the residual cover whole lines (512 bytes of a row per wave
 //     and load), and the activation's code exists once, in a loop, not once per accumulator element.
 // What bounds it: the matrix unit is busy for half of the cycles, the rest is what one wave per SIMD issues beside it, as in the
-// plain kernel.  Gate and up of 4096 -> 11008, 2048 rows 380 us (972 TF/s); the same by 8 experts, 4096 rows 863 us (856 TF/s; every
+// plain kernel.  Gate and up of 4096 -> 11008, 2048 rows 371 us (995 TF/s); the same by 8 experts, 4096 rows 839 us (881 TF/s; every
 // expert ends in a tile that is not full).
 template <bool kGated>
 struct GemmOpsPlace {

@@ -18,7 +18,7 @@
 // What bounds it: decoding, on the vector ALU (half of the cycles) and the LDS (45 %; four gathers of 16 bytes per two codes, no bank
 // conflicts), beside 18 % on the matrix unit: 11008 -> 4096 by 16 experts, 48 rows on 15 of them 56.0 us, 169 MB of codes at
 // 3.0 TB/s; one matrix and few rows: a launch, a pass of the tables and one or two steps per wave (13 rows, 4096 -> 11007, GELU,
-// 7.5 us).
+// 7.3 us).
 // LDS map: tables [0, 96K), then W pieces of XI KB.
 struct OpsCursor {
     int expert, row, row_end;   // segment: rows row .. of an expert whose rows end at row_end
@@ -211,8 +211,8 @@ __device__ __forceinline__ OpsRowsArgs rows_args_copy()
 // computed, and left to the 16-bit body in the same launch, with the same jobs: all of them if the grid does not fit
 // fp8 (known before the first), and those that met an x that is not finite (the terms of an infinity mean
 // nothing), which store nothing here.
-// What bounds it: the vector ALU, two thirds of the cycles (gate and up of 8192 -> 28672, one row, 30.8 us, 3.8 TB/s of codes; of 4096 ->
-// 11008 by two of eight experts, one row each, 17.9 us, 2.5 TB/s).
+// What bounds it: the vector ALU, two thirds of the cycles (gate and up of 8192 -> 28672, one row, 30.2 us, 3.9 TB/s of codes; of 4096 ->
+// 11008 by two of eight experts, one row each, 17.8 us, 2.5 TB/s).
 constexpr int kO8TermPitch = 272, kO8MeanPitch = 80;
 constexpr int kO8Means = 8 * kO8TermPitch;
 constexpr int kO8Piece = kO8Means + 4 * kO8MeanPitch + 64;   // 2560
