@@ -6,8 +6,8 @@
 // Lane l of them holds logits l, L + l, ... of the row as ordered unsigned keys (equal numbers have equal keys, -inf and
 // NaN have key 0 and are never chosen); k times the largest key is found with a maximum over the lanes, then the
 // lowest index that holds it.  Lane j keeps choice j.  The vector ALU bounds it: sixteen lanes per token take a
-// fifth of the instructions per token that a wave per token took.  16384 tokens, 8 of 128 experts: 14.2 us for both kernels, 8.7 and
-// 6.7 by the trace; 24 tokens, 2 of 16, one launch: 5.1 us a call, 2.8 by the trace.
+// fifth of the instructions per token that a wave per token took.  16384 tokens, 8 of 128 experts: 14.2 us for both kernels, 9 and
+// 7 by the trace; 24 tokens, 2 of 16, one launch: 5.1 us a call, 2.8 by the trace.
 //
 // The lists.  Sorting by expert must keep the order of the tokens, and within a token an expert is chosen
 // once, so a row's place is: first row of its expert + number of earlier tokens that chose the expert.  A workgroup
